@@ -73,11 +73,13 @@ const char* ilqr_b200_status_string(int status) {
   switch (status) {
     case ILQR_OK: return "ok";
     case ILQR_ERR_INVALID_ARGUMENT: return "invalid argument (null pointer, size or step sizes)";
-    case ILQR_ERR_MISALIGNED: return "C / grad_C must be 16-byte aligned";
+    case ILQR_ERR_MISALIGNED: return "C / grad_C must be 16-byte aligned, other tensors and workspaces to their type";
     case ILQR_ERR_WORKSPACE: return "workspace missing or too small";
     case ILQR_ERR_CUDA: return "CUDA launch or driver entry point failure";
     case ILQR_ERR_UNSUPPORTED_DEVICE: return "device is not compute capability 10.0 (B200)";
     case ILQR_ERR_NOALLOC_LIMIT: return "problem too large for the fixed scratch of the no-allocation entry point";
+    case ILQR_ERR_OVERLAP: return "an output shares memory with another tensor of the call";
+    case ILQR_ERR_HOST_MEMORY: return "out of host memory";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,579 @@
+// ilqr_gradclip.cu -- norms of gradients and clipping by them.
+//
+// Over a list of tensors: n = sqrt(sum g^2) (or max |g|), c = min(1, m / (n + eps)),
+// out = c g. Per batch element: the same over each element's slices of up to
+// eight tensors.
+//
+// Sums: eight values are squared and added in 32 bits, and those sums in 64
+// bits. Eight roundings of relative size 2^-24 at most move a sum of squares by
+// 2^-21, its root by 2^-22, whatever the length. Squares that leave the range
+// of a float (|g| above 2^63, or so small that the group's sum is under 2^-100)
+// are formed again in 64 bits, so a norm is right wherever it is a float
+// itself. The order of every sum is fixed by sizes and grid: no atomics, the
+// same bits each time.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ilqr_b200.h"
+#include "ilqr_gradclip.h"
+
+namespace ilqr {
+
+namespace {
+
+constexpr int NT = 256;  // threads of a block
+constexpr int UN = 4;    // 16-byte loads that a thread has in flight
+
+// ---- values ----------------------------------------------------------------
+
+template <int DT> struct Type;
+template <> struct Type<ILQR_DTYPE_F32> {
+  static constexpr int SIZE = 4;
+  static constexpr bool WIDE = true;  // squares can leave the range of a float
+};
+template <> struct Type<ILQR_DTYPE_F16> {
+  static constexpr int SIZE = 2;
+  static constexpr bool WIDE = false;
+};
+template <> struct Type<ILQR_DTYPE_BF16> {
+  static constexpr int SIZE = 2;
+  static constexpr bool WIDE = true;
+};
+
+// the values of one 32-bit word
+template <int DT>
+__device__ __forceinline__ void unpack(uint32_t w, float* x) {
+  if constexpr (DT == ILQR_DTYPE_F32) {
+    x[0] = __uint_as_float(w);
+  } else if constexpr (DT == ILQR_DTYPE_BF16) {
+    x[0] = __uint_as_float(w << 16);
+    x[1] = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x[0] = f.x;
+    x[1] = f.y;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack(const float* x) {
+  if constexpr (DT == ILQR_DTYPE_F32) {
+    return __float_as_uint(x[0]);
+  } else if constexpr (DT == ILQR_DTYPE_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[0], x[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(x[0], x[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ float load_one(const char* p) {
+  if constexpr (DT == ILQR_DTYPE_F32) return *reinterpret_cast<const float*>(p);
+  if constexpr (DT == ILQR_DTYPE_BF16) return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
+  return __half2float(*reinterpret_cast<const __half*>(p));
+}
+
+template <int DT>
+__device__ __forceinline__ void store_one(char* p, float x) {
+  if constexpr (DT == ILQR_DTYPE_F32) *reinterpret_cast<float*>(p) = x;
+  else if constexpr (DT == ILQR_DTYPE_BF16) *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(x);
+  else *reinterpret_cast<__half*>(p) = __float2half_rn(x);
+}
+
+// ---- sums ------------------------------------------------------------------
+
+// MAX: the largest magnitude, kept as its bits: those order magnitudes as
+// integers, with NaN above infinity, so a NaN stays the largest.
+template <bool MAX> struct Acc {
+  double s = 0.0;
+};
+template <> struct Acc<true> {
+  uint32_t m = 0u;
+};
+
+template <int DT, int N>
+__device__ __forceinline__ void add(Acc<false>& a, const float* x) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s = __fmaf_rn(x[i], x[i], s);
+  if (!Type<DT>::WIDE || (s >= 0x1p-100f && s < __int_as_float(0x7f800000))) {
+    a.s += (double)s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.s = __fma_rn((double)x[i], (double)x[i], a.s);
+  }
+}
+
+template <int DT, int N>
+__device__ __forceinline__ void add(Acc<true>& a, const float* x) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.m = max(a.m, __float_as_uint(x[i]) & 0x7fffffffu);
+}
+
+__device__ __forceinline__ double value(const Acc<false>& a) { return a.s; }
+__device__ __forceinline__ double value(const Acc<true>& a) { return (double)__uint_as_float(a.m); }
+
+template <bool MAX>
+__device__ __forceinline__ double join(double a, double b) {
+  if constexpr (!MAX) return a + b;
+  return a != a ? a : (b != b || b > a ? b : a);
+}
+
+template <bool MAX>
+__device__ __forceinline__ double warp_join(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = join<MAX>(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The join over a block, for every thread; sh has a place for each warp.
+template <bool MAX>
+__device__ __forceinline__ double block_join(double v, double* sh) {
+  v = warp_join<MAX>(v);
+  __syncthreads();  // sh may still be read from the join before
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < (blockDim.x >> 5) ? sh[threadIdx.x & 31] : 0.0;
+  return warp_join<MAX>(v);
+}
+
+__device__ __forceinline__ double norm_of(double total, bool max_type) { return max_type ? total : sqrt(total); }
+
+struct Coef {
+  float f;
+  double d;
+  bool wide;  // f is so small that it has lost bits: the product is formed in 64 bits
+};
+
+__device__ __forceinline__ Coef coef_of(double norm, double max_norm, double eps) {
+  Coef c;
+  c.d = max_norm / (norm + eps);
+  if (c.d >= 1.0 || isinf(max_norm)) c.d = 1.0;  // NaN stays
+  c.f = (float)c.d;
+  c.wide = c.d < 0x1p-100;
+  return c;
+}
+
+__device__ __forceinline__ float scaled(float x, const Coef& c) {
+  return c.wide ? (float)((double)x * c.d) : x * c.f;
+}
+
+// ---- a range of a dense tensor ---------------------------------------------
+
+__device__ __forceinline__ uint4 load16(const char* p) { return *reinterpret_cast<const uint4*>(p); }
+
+template <int DT>
+__device__ __forceinline__ int head_of(const char* p, int64_t n) {
+  const int h = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / Type<DT>::SIZE;
+  return n < h ? (int)n : h;
+}
+
+template <int DT, bool MAX>
+__device__ __forceinline__ void add_vec(Acc<MAX>& a, const uint4& v) {
+  float x[8];
+  if constexpr (DT == ILQR_DTYPE_F32) {
+    unpack<DT>(v.x, x), unpack<DT>(v.y, x + 1), unpack<DT>(v.z, x + 2), unpack<DT>(v.w, x + 3);
+    add<DT, 4>(a, x);
+  } else {
+    unpack<DT>(v.x, x), unpack<DT>(v.y, x + 2), unpack<DT>(v.z, x + 4), unpack<DT>(v.w, x + 6);
+    add<DT, 8>(a, x);
+  }
+}
+
+template <int DT, bool MAX>
+__device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n) {
+  constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
+  const int tid = threadIdx.x;
+  const int h = head_of<DT>(p, n);
+  if (tid < h) {
+    const float x = load_one<DT>(p + tid * SZ);
+    add<DT, 1>(a, &x);
+  }
+  p += h * SZ;
+  n -= h;
+  const int64_t nv = n / VE;
+  for (int64_t i = tid; i < nv; i += UN * NT) {
+    uint4 v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (i + u * NT < nv) v[u] = load16(p + (i + u * NT) * 16);
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (i + u * NT < nv) add_vec<DT, MAX>(a, v[u]);
+  }
+  const int tail = (int)(n - nv * VE);
+  if (tid < tail) {
+    const float x = load_one<DT>(p + (nv * VE + tid) * SZ);
+    add<DT, 1>(a, &x);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 scale_vec(const uint4& v, const Coef& c) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float x[2];
+    unpack<DT>(w[k], x);
+#pragma unroll
+    for (int j = 0; j < 4 / Type<DT>::SIZE; ++j) x[j] = scaled(x[j], c);
+    w[k] = pack<DT>(x);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// out = c in; `in` may be `out`
+template <int DT>
+__device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c) {
+  constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
+  const int tid = threadIdx.x;
+  const int h = head_of<DT>(p, n);
+  if (tid < h) store_one<DT>(q + tid * SZ, scaled(load_one<DT>(p + tid * SZ), c));
+  p += h * SZ;
+  q += h * SZ;
+  n -= h;
+  const bool together = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
+  const int64_t nv = n / VE;
+  for (int64_t i = tid; i < nv; i += UN * NT) {
+    uint4 v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (i + u * NT < nv) v[u] = load16(p + (i + u * NT) * 16);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (i + u * NT >= nv) continue;
+      const uint4 y = scale_vec<DT>(v[u], c);
+      char* to = q + (i + u * NT) * 16;
+      if (together) {
+        *reinterpret_cast<uint4*>(to) = y;
+      } else {
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (SZ == 4) {
+            reinterpret_cast<uint32_t*>(to)[k] = w[k];
+          } else {
+            reinterpret_cast<uint16_t*>(to)[2 * k] = (uint16_t)w[k];
+            reinterpret_cast<uint16_t*>(to)[2 * k + 1] = (uint16_t)(w[k] >> 16);
+          }
+        }
+      }
+    }
+  }
+  const int tail = (int)(n - nv * VE);
+  if (tid < tail) {
+    const int64_t at = (nv * VE + tid) * SZ;
+    store_one<DT>(q + at, scaled(load_one<DT>(p + at), c));
+  }
+}
+
+// ---- lists -----------------------------------------------------------------
+
+// The tensor that chunk k belongs to.
+template <int CAP>
+__device__ __forceinline__ int find(const GradTable<CAP>& tab, uint32_t k) {
+  int lo = 0, hi = tab.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.e[mid].chunk0 <= k) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint32_t first_chunk(uint32_t block, uint32_t chunks, uint32_t grid) {
+  return (uint32_t)((uint64_t)block * chunks / grid);
+}
+
+// the block whose chunks [first_chunk(b), first_chunk(b + 1)) hold chunk k
+__device__ __forceinline__ uint32_t block_of(uint32_t k, uint32_t chunks, uint32_t grid) {
+  return (uint32_t)((((uint64_t)k + 1) * grid - 1) / chunks);
+}
+
+template <int CAP>
+__device__ __forceinline__ void span(const GradTable<CAP>& tab, int t, uint32_t k0, uint32_t k1, int64_t* at,
+                                     int64_t* n) {
+  const GradEntry& e = tab.e[t];
+  const int64_t per = tab.chunk_bytes / (e.dtype == ILQR_DTYPE_F32 ? 4 : 2);
+  const int64_t a = (int64_t)(k0 - e.chunk0) * per, b = (int64_t)(k1 - e.chunk0) * per;
+  *at = a;
+  *n = (b < e.numel ? b : e.numel) - a;
+}
+
+template <bool MAX>
+__device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const void* in, int64_t at, int64_t n) {
+  const char* p = static_cast<const char*>(in);
+  if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX>(a, p + at * 4, n);
+  else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX>(a, p + at * 2, n);
+  else range_sum<ILQR_DTYPE_F16, MAX>(a, p + at * 2, n);
+}
+
+// Partial sums. Each block takes a contiguous run of chunks; with PER one sum
+// for each tensor in it, at slot block + tensor: slots of neighbours are
+// neighbours, and where a block ends with its tensor the one slot that falls
+// out is set to 0, the identity of both joins.
+template <int CAP, bool MAX, bool PER>
+__global__ void __launch_bounds__(NT) grad_sum_kernel(const __grid_constant__ GradTable<CAP> tab, double* slots) {
+  __shared__ double sh[32];
+  asm volatile("griddepcontrol.launch_dependents;");
+  uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
+  const uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
+  int t = find(tab, k);
+  if (PER && blockIdx.x > 0 && k == tab.e[t].chunk0 && threadIdx.x == 0) slots[blockIdx.x + t - 1] = 0.0;
+  Acc<MAX> a;
+  for (; k < k1; ++t) {
+    const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
+    int64_t at, n;
+    span(tab, t, k, end, &at, &n);
+    entry_sum<MAX>(a, tab.e[t].dtype, tab.e[t].in, at, n);
+    if (PER) {
+      const double v = block_join<MAX>(value(a), sh);
+      if (threadIdx.x == 0) slots[blockIdx.x + t] = v;
+      a = Acc<MAX>();
+    }
+    k = end;
+  }
+  if (!PER) {
+    const double v = block_join<MAX>(value(a), sh);
+    if (threadIdx.x == 0) slots[blockIdx.x] = v;
+  }
+}
+
+template <bool MAX>
+__device__ __forceinline__ double join_slots(const double* slots, int64_t n, double* sh) {
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) v = join<MAX>(v, slots[i]);
+  return block_join<MAX>(v, sh);
+}
+
+// Block 0: the norm of the whole list. The others: a warp for each tensor.
+template <int CAP, bool MAX>
+__global__ void __launch_bounds__(NT) grad_join_kernel(const __grid_constant__ GradTable<CAP> tab, uint32_t grid,
+                                                       const double* tab_slots, const double* slots, int64_t n_slots,
+                                                       GradNormOut out, int want_global) {
+  __shared__ double sh[32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x == 0) {
+    if (!want_global) return;
+    const double v = join_slots<MAX>(slots, n_slots, sh);
+    if (threadIdx.x == 0) {
+      if (out.norm != nullptr) *out.norm = (float)norm_of(v, MAX);
+      if (out.total != nullptr) *out.total = v;
+    }
+    return;
+  }
+  const int t = (int)(blockIdx.x - 1) * (NT / 32) + (int)(threadIdx.x >> 5);
+  if (t >= tab.n) return;
+  const uint32_t c0 = tab.e[t].chunk0, c1 = t + 1 < tab.n ? tab.e[t + 1].chunk0 : tab.chunks;
+  const uint32_t lo = block_of(c0, tab.chunks, grid) + t, hi = block_of(c1 - 1, tab.chunks, grid) + t;
+  double v = 0.0;
+  for (uint32_t i = lo + (threadIdx.x & 31); i <= hi; i += 32) v = join<MAX>(v, tab_slots[i]);
+  v = warp_join<MAX>(v);
+  if ((threadIdx.x & 31) == 0) out.tensor_norms[t] = (float)norm_of(v, MAX);
+}
+
+// out = c in over the list; every block joins the partial sums for itself, in
+// the same order. In place a coefficient of 1 leaves the values where they are.
+template <int CAP>
+__global__ void __launch_bounds__(NT) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
+                                                        const double* slots, int64_t n_slots, float* norm) {
+  __shared__ double sh[32];
+  uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
+  const uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
+  int t = find(tab, k);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double total = s.max_type ? join_slots<true>(slots, n_slots, sh) : join_slots<false>(slots, n_slots, sh);
+  const double nrm = norm_of(total, s.max_type);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
+  const Coef c = coef_of(nrm, s.max_norm, s.eps);
+  for (; k < k1; ++t) {
+    const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
+    const GradEntry& e = tab.e[t];
+    if (!(c.d == 1.0 && e.in == e.out)) {
+      int64_t at, n;
+      span(tab, t, k, end, &at, &n);
+      const char* p = static_cast<const char*>(e.in);
+      char* q = static_cast<char*>(e.out);
+      if (e.dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p + at * 4, q + at * 4, n, c);
+      else if (e.dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p + at * 2, q + at * 2, n, c);
+      else range_scale<ILQR_DTYPE_F16>(p + at * 2, q + at * 2, n, c);
+    }
+    k = end;
+  }
+}
+
+// ---- batch elements ---------------------------------------------------------
+
+template <int VB> struct Vec;
+template <> struct Vec<16> { uint4 w; };
+template <> struct Vec<8> { uint2 w; };
+template <> struct Vec<4> { uint32_t w; };
+template <> struct Vec<2> { uint16_t w; };
+
+template <int DT, int VB>
+__device__ __forceinline__ void unpack_vec(const Vec<VB>& v, float* x) {
+  if constexpr (VB == 2) {
+    unpack<DT>((uint32_t)v.w, x);
+  } else {
+    constexpr int K = 4 / Type<DT>::SIZE;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < VB / 4; ++k) unpack<DT>(w[k], x + k * K);
+  }
+}
+
+template <int DT, int VB>
+__device__ __forceinline__ Vec<VB> pack_vec(const float* x) {
+  Vec<VB> v;
+  if constexpr (VB == 2) {
+    const float two[2] = {x[0], 0.0f};
+    v.w = (uint16_t)pack<DT>(two);
+  } else {
+    constexpr int K = 4 / Type<DT>::SIZE;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < VB / 4; ++k) w[k] = pack<DT>(x + k * K);
+  }
+  return v;
+}
+
+template <int DT, int VB>
+__device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, uint32_t lane, uint32_t step) {
+  constexpr int NV = VB / Type<DT>::SIZE;
+  const char* p = r.in + b * r.in_row;
+  const uint32_t n = r.n_seg * r.seg_vecs;
+  for (uint32_t i = lane; i < n; i += step) {
+    const uint32_t s = r.n_seg == 1 ? 0 : i / r.seg_vecs;
+    float x[NV < 2 ? 2 : NV];
+    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(p + s * r.in_seg + (int64_t)(i - s * r.seg_vecs) * VB), x);
+    add<DT, NV>(a, x);
+  }
+}
+
+template <int DT, int VB>
+__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const Coef& c, bool zero, uint32_t lane,
+                                          uint32_t step) {
+  constexpr int NV = VB / Type<DT>::SIZE;
+  const char* p = r.in + b * r.in_row;
+  char* q = r.out + b * r.out_row;
+  const uint32_t n = r.n_seg * r.seg_vecs;
+  for (uint32_t i = lane; i < n; i += step) {
+    const uint32_t s = r.n_seg == 1 ? 0 : i / r.seg_vecs;
+    const int64_t off = (int64_t)(i - s * r.seg_vecs) * VB;
+    float x[NV < 2 ? 2 : NV];
+    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(p + s * r.in_seg + off), x);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j] = zero ? 0.0f : scaled(x[j], c);
+    *reinterpret_cast<Vec<VB>*>(q + s * r.out_seg + off) = pack_vec<DT, VB>(x);
+  }
+}
+
+#define ROW_DISPATCH(r, CALL)                                                       \
+  switch ((r).dtype * 32 + (r).vec_bytes) {                                         \
+    case ILQR_DTYPE_F32 * 32 + 16: CALL(ILQR_DTYPE_F32, 16); break;                 \
+    case ILQR_DTYPE_F32 * 32 + 8: CALL(ILQR_DTYPE_F32, 8); break;                   \
+    case ILQR_DTYPE_F32 * 32 + 4: CALL(ILQR_DTYPE_F32, 4); break;                   \
+    case ILQR_DTYPE_F16 * 32 + 16: CALL(ILQR_DTYPE_F16, 16); break;                 \
+    case ILQR_DTYPE_F16 * 32 + 8: CALL(ILQR_DTYPE_F16, 8); break;                   \
+    case ILQR_DTYPE_F16 * 32 + 4: CALL(ILQR_DTYPE_F16, 4); break;                   \
+    case ILQR_DTYPE_F16 * 32 + 2: CALL(ILQR_DTYPE_F16, 2); break;                   \
+    case ILQR_DTYPE_BF16 * 32 + 16: CALL(ILQR_DTYPE_BF16, 16); break;               \
+    case ILQR_DTYPE_BF16 * 32 + 8: CALL(ILQR_DTYPE_BF16, 8); break;                 \
+    case ILQR_DTYPE_BF16 * 32 + 4: CALL(ILQR_DTYPE_BF16, 4); break;                 \
+    default: CALL(ILQR_DTYPE_BF16, 2); break;                                       \
+  }
+
+// A warp (ONE_WARP) or a block for each element.
+template <bool ONE_WARP>
+__global__ void __launch_bounds__(NT) grad_rows_kernel(const __grid_constant__ RowTable tab) {
+  __shared__ double sh[32];
+  const int64_t b = ONE_WARP ? (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (b >= tab.B) return;
+  const uint32_t lane = ONE_WARP ? threadIdx.x & 31 : threadIdx.x;
+  constexpr uint32_t step = ONE_WARP ? 32 : NT;
+  Acc<false> a;
+  for (int k = 0; k < tab.n; ++k) {
+    const RowTensor& r = tab.t[k];
+#define CALL(DT, VB) row_sum<DT, VB>(a, r, b, lane, step)
+    ROW_DISPATCH(r, CALL)
+#undef CALL
+  }
+  const double nrm = sqrt(ONE_WARP ? warp_join<false>(a.s) : block_join<false>(a.s, sh));
+  if (lane == 0 && tab.norms != nullptr) tab.norms[b] = (float)nrm;
+  const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
+  const bool zero = tab.zero_nonfinite && !isfinite(nrm);
+  for (int k = 0; k < tab.n; ++k) {
+    const RowTensor& r = tab.t[k];
+    if (c.d == 1.0 && !zero && r.in == r.out) continue;
+#define CALL(DT, VB) row_scale<DT, VB>(r, b, c, zero, lane, step)
+    ROW_DISPATCH(r, CALL)
+#undef CALL
+  }
+}
+
+// ---- launches ---------------------------------------------------------------
+
+template <typename... K, typename... A>
+cudaError_t launch(void (*kernel)(K...), unsigned grid, bool dependent, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(NT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...);
+}
+
+}  // namespace
+
+template <int CAP>
+cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, bool per_tensor, double* slots,
+                            cudaStream_t stream) {
+  if (max_type)
+    return per_tensor ? launch(grad_sum_kernel<CAP, true, true>, grid, false, stream, tab, slots)
+                      : launch(grad_sum_kernel<CAP, true, false>, grid, false, stream, tab, slots);
+  return per_tensor ? launch(grad_sum_kernel<CAP, false, true>, grid, false, stream, tab, slots)
+                    : launch(grad_sum_kernel<CAP, false, false>, grid, false, stream, tab, slots);
+}
+
+template <int CAP>
+cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* tab_slots, bool max_type,
+                             const double* slots, int64_t n_slots, const GradNormOut& out, bool want_global,
+                             cudaStream_t stream) {
+  static const GradTable<CAP> none{};
+  const unsigned blocks = 1 + (tab != nullptr ? (unsigned)(tab->n + NT / 32 - 1) / (NT / 32) : 0);
+  const GradTable<CAP>& use = tab != nullptr ? *tab : none;
+  return max_type ? launch(grad_join_kernel<CAP, true>, blocks, true, stream, use, (uint32_t)grid, tab_slots, slots,
+                           n_slots, out, want_global ? 1 : 0)
+                  : launch(grad_join_kernel<CAP, false>, blocks, true, stream, use, (uint32_t)grid, tab_slots, slots,
+                           n_slots, out, want_global ? 1 : 0);
+}
+
+template <int CAP>
+cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
+                              int64_t n_slots, float* norm, bool dependent, cudaStream_t stream) {
+  return launch(grad_scale_kernel<CAP>, grid, dependent, stream, tab, s, slots, n_slots, norm);
+}
+
+#define INSTANTIATE(CAP)                                                                                              \
+  template cudaError_t launch_grad_sum<CAP>(const GradTable<CAP>&, int, bool, bool, double*, cudaStream_t);           \
+  template cudaError_t launch_grad_join<CAP>(const GradTable<CAP>*, int, const double*, bool, const double*, int64_t, \
+                                             const GradNormOut&, bool, cudaStream_t);                                 \
+  template cudaError_t launch_grad_scale<CAP>(const GradTable<CAP>&, int, const GradScale&, const double*, int64_t,   \
+                                              float*, bool, cudaStream_t);
+INSTANTIATE(GRAD_CAP_SHORT)
+INSTANTIATE(GRAD_CAP_LONG)
+#undef INSTANTIATE
+
+cudaError_t launch_grad_rows(const RowTable& tab, int64_t row_bytes, cudaStream_t stream) {
+  if (row_bytes <= 4096)
+    return launch(grad_rows_kernel<true>, (unsigned)((tab.B + NT / 32 - 1) / (NT / 32)), false, stream, tab);
+  return launch(grad_rows_kernel<false>, (unsigned)tab.B, false, stream, tab);
+}
+
+}  // namespace ilqr

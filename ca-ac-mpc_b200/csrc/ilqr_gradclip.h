@@ -1,0 +1,91 @@
+// ilqr_gradclip.h -- launch records of the gradient norm and clipping kernels
+// (ilqr_gradclip.cu), filled by the entry points in ilqr_gradclip_abi.cu.
+#ifndef ILQR_GRADCLIP_H
+#define ILQR_GRADCLIP_H
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace ilqr {
+
+// One dense tensor of a list: its values are cut into chunks of chunk_bytes,
+// numbered through the list; chunk0 is its first. Every tensor has at least
+// one chunk (an empty one, a chunk without values).
+struct GradEntry {
+  const void* in;
+  void* out;
+  int64_t numel;
+  uint32_t chunk0;
+  uint32_t dtype;
+};
+
+// Kernel parameters hold at most 32764 bytes: longer lists take several
+// launches. The short table keeps the usual call's parameter copy small.
+constexpr int GRAD_CAP_SHORT = 60;
+constexpr int GRAD_CAP_LONG = 1000;
+
+template <int CAP>
+struct GradTable {
+  int32_t n;
+  uint32_t chunks;
+  uint32_t chunk_bytes;
+  uint32_t pad;
+  GradEntry e[CAP];
+};
+
+// Partial sums of a launch: one per block, or with per-tensor sums one per
+// (block, tensor) that meet, at slot block + tensor.
+constexpr int GRAD_MAX_GRID = 148 * 8;
+constexpr uint32_t GRAD_CHUNK_BYTES = 16384;
+
+struct GradNormOut {
+  float* norm;          // may be null
+  float* tensor_norms;  // may be null
+  double* total;        // may be null
+};
+
+struct GradScale {
+  double max_norm;
+  double eps;
+  int32_t max_type;  // 1: largest magnitude, 0: 2-norm
+};
+
+// One tensor of the per-element form: row b is n_seg segments of seg_vecs
+// vectors of vec_bytes; strides in bytes.
+struct RowTensor {
+  const char* in;
+  char* out;
+  int64_t in_row, in_seg, out_row, out_seg;
+  uint32_t n_seg, seg_vecs;
+  uint32_t vec_bytes, dtype;
+};
+
+constexpr int ROW_MAX_TENSORS = 8;
+
+struct RowTable {
+  RowTensor t[ROW_MAX_TENSORS];
+  int32_t n;
+  int32_t zero_nonfinite;
+  int64_t B;
+  double max_norm, eps;
+  float* norms;
+};
+
+template <int CAP>
+cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, bool per_tensor, double* slots,
+                            cudaStream_t stream);
+// Joins n_slots partials into the norm; with tab != nullptr also the norms of
+// its tensors from the launch's own slots (tab_slots, grid).
+template <int CAP>
+cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* tab_slots, bool max_type,
+                             const double* slots, int64_t n_slots, const GradNormOut& out, bool want_global,
+                             cudaStream_t stream);
+template <int CAP>
+cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
+                              int64_t n_slots, float* norm, bool dependent, cudaStream_t stream);
+cudaError_t launch_grad_rows(const RowTable& tab, int64_t row_bytes, cudaStream_t stream);
+
+}  // namespace ilqr
+
+#endif

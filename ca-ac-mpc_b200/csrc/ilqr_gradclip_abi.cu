@@ -1,0 +1,335 @@
+// ilqr_gradclip_abi.cu -- extern "C" entry points of the gradient norms and
+// clipping (include/ilqr_b200.h). The host arrays that describe the tensors
+// are read during the call only: what the kernels need of them travels in the
+// launch parameters, so a captured call keeps nothing of the caller's.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "ilqr_b200.h"
+#include "ilqr_gradclip.h"
+
+namespace {
+
+using ilqr::GradEntry;
+using ilqr::GradTable;
+
+int status_of(cudaError_t e) { return e == cudaSuccess ? ILQR_OK : ILQR_ERR_CUDA; }
+
+int64_t size_of(int32_t dtype) { return dtype == ILQR_DTYPE_F32 ? 4 : 2; }
+
+constexpr int64_t MAX_VALUES = (int64_t)1 << 40;  // of a list: chunk numbers stay in 32 bits
+
+struct List {
+  const void* const* in;
+  void* const* out;  // nullptr: norm only
+  const int64_t* numel;
+  const int32_t* dtype;
+  int32_t n;
+};
+
+int check_list(const List& l, int32_t norm_type) {
+  if (l.n < 0 || (norm_type != ILQR_NORM_L2 && norm_type != ILQR_NORM_MAX)) return ILQR_ERR_INVALID_ARGUMENT;
+  if (l.n > 0 && (l.in == nullptr || l.numel == nullptr || l.dtype == nullptr)) return ILQR_ERR_INVALID_ARGUMENT;
+  int64_t values = 0;
+  for (int32_t i = 0; i < l.n; ++i) {
+    if (l.dtype[i] < ILQR_DTYPE_F32 || l.dtype[i] > ILQR_DTYPE_BF16) return ILQR_ERR_INVALID_ARGUMENT;
+    if (l.numel[i] < 0 || l.numel[i] > MAX_VALUES) return ILQR_ERR_INVALID_ARGUMENT;
+    values += l.numel[i];
+    if (values > MAX_VALUES) return ILQR_ERR_INVALID_ARGUMENT;
+    if (l.numel[i] == 0) continue;
+    const uintptr_t low = (uintptr_t)size_of(l.dtype[i]) - 1;
+    if (l.in[i] == nullptr || (l.out != nullptr && l.out[i] == nullptr)) return ILQR_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)l.in[i] & low) || (l.out != nullptr && ((uintptr_t)l.out[i] & low))) return ILQR_ERR_MISALIGNED;
+  }
+  return ILQR_OK;
+}
+
+struct Span {
+  uintptr_t lo, hi;
+  int32_t tensor;
+  bool out;
+};
+
+// Whether a value that the call writes is also one that it writes or reads
+// elsewhere: blocks run in no order, so only a tensor's own input may be its
+// output, whole.
+bool overlaps(const List& l) {
+  std::vector<Span> s;
+  s.reserve(2 * (size_t)l.n);
+  for (int32_t i = 0; i < l.n; ++i) {
+    if (l.numel[i] == 0) continue;
+    const uintptr_t bytes = (uintptr_t)(l.numel[i] * size_of(l.dtype[i]));
+    const uintptr_t q = (uintptr_t)l.out[i], p = (uintptr_t)l.in[i];
+    s.push_back({q, q + bytes, i, true});
+    if (p != q) s.push_back({p, p + bytes, i, false});
+  }
+  const auto before = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
+  uintptr_t end_out = 0, end_any = 0;  // of the spans before this one
+  for (const Span& x : s) {
+    if (x.lo < (x.out ? end_any : end_out)) return true;
+    end_any = std::max(end_any, x.hi);
+    if (x.out) end_out = std::max(end_out, x.hi);
+  }
+  return false;
+}
+
+uint64_t chunks_of(int64_t numel, int32_t dtype) {
+  const uint64_t c = ((uint64_t)(numel * size_of(dtype)) + ilqr::GRAD_CHUNK_BYTES - 1) / ilqr::GRAD_CHUNK_BYTES;
+  return c > 0 ? c : 1;
+}
+
+template <int CAP>
+void fill(GradTable<CAP>& tab, const List& l, int32_t first, int32_t n) {
+  tab.n = n;
+  tab.chunk_bytes = ilqr::GRAD_CHUNK_BYTES;
+  tab.pad = 0;
+  uint64_t at = 0;
+  for (int32_t i = 0; i < n; ++i) {
+    const int32_t k = first + i;
+    tab.e[i] = GradEntry{l.in[k], l.out != nullptr ? l.out[k] : nullptr, l.numel[k], (uint32_t)at,
+                         (uint32_t)l.dtype[k]};
+    at += chunks_of(l.numel[k], l.dtype[k]);
+  }
+  tab.chunks = (uint32_t)at;
+}
+
+int grid_of(uint32_t chunks) { return (int)std::min<uint32_t>(chunks, (uint32_t)ilqr::GRAD_MAX_GRID); }
+
+// Slots that the partial sums of a list take, at most.
+size_t slots_of(int32_t n) {
+  const size_t launches = ((size_t)n + ilqr::GRAD_CAP_LONG - 1) / ilqr::GRAD_CAP_LONG;
+  return launches * ilqr::GRAD_MAX_GRID + (size_t)n + 1;  // and one for the joined total
+}
+
+constexpr int64_t MANY_SLOTS = 4096;  // beyond this the blocks of the scaling do not each join them
+
+template <int CAP>
+int norm_impl(const List& l, bool max_type, const ilqr::GradNormOut& o, double* slots, cudaStream_t stream) {
+  const std::unique_ptr<GradTable<CAP>> tab(new GradTable<CAP>);
+  const bool per = o.tensor_norms != nullptr;
+  int64_t used = 0;
+  for (int32_t first = 0; first < l.n; first += CAP) {
+    const int32_t n = std::min<int32_t>(CAP, l.n - first);
+    fill(*tab, l, first, n);
+    const int grid = grid_of(tab->chunks);
+    cudaError_t e = ilqr::launch_grad_sum(*tab, grid, max_type, per, slots + used, stream);
+    if (e != cudaSuccess) return ILQR_ERR_CUDA;
+    const double* mine = slots + used;
+    used += grid + (per ? n - 1 : 0);
+    const bool last = first + n == l.n;
+    if (per || last) {
+      ilqr::GradNormOut part = o;
+      if (per) part.tensor_norms = o.tensor_norms + first;
+      e = ilqr::launch_grad_join<CAP>(per ? tab.get() : nullptr, grid, mine, max_type, slots, used, part, last, stream);
+      if (e != cudaSuccess) return ILQR_ERR_CUDA;
+    }
+  }
+  return ILQR_OK;
+}
+
+template <int CAP>
+int clip_impl(const List& l, const ilqr::GradScale& s, const double* total, float* norm, double* slots,
+              cudaStream_t stream) {
+  const std::unique_ptr<GradTable<CAP>> tab(new GradTable<CAP>);
+  const double* from = total;
+  int64_t used = 1;
+  if (total == nullptr) {
+    used = 0;
+    for (int32_t first = 0; first < l.n; first += CAP) {
+      fill(*tab, l, first, std::min<int32_t>(CAP, l.n - first));
+      const int grid = grid_of(tab->chunks);
+      if (ilqr::launch_grad_sum(*tab, grid, s.max_type != 0, false, slots + used, stream) != cudaSuccess)
+        return ILQR_ERR_CUDA;
+      used += grid;
+    }
+    from = slots;
+    if (used > MANY_SLOTS) {
+      const ilqr::GradNormOut o{nullptr, nullptr, slots + used};
+      if (ilqr::launch_grad_join<CAP>(nullptr, 0, nullptr, s.max_type != 0, slots, used, o, true, stream) !=
+          cudaSuccess)
+        return ILQR_ERR_CUDA;
+      from = slots + used;
+      used = 1;
+    }
+  }
+  for (int32_t first = 0; first < l.n; first += CAP) {
+    if (l.n > CAP || total != nullptr) fill(*tab, l, first, std::min<int32_t>(CAP, l.n - first));
+    if (ilqr::launch_grad_scale(*tab, grid_of(tab->chunks), s, from, used, first == 0 ? norm : nullptr,
+                                total == nullptr, stream) != cudaSuccess)
+      return ILQR_ERR_CUDA;
+  }
+  return ILQR_OK;
+}
+
+int64_t magnitude(int64_t v) { return v < 0 ? -v : v; }
+
+}  // namespace
+
+extern "C" {
+
+int ilqr_b200_grad_workspace_size(int32_t n_tensors, size_t* bytes) {
+  if (bytes == nullptr || n_tensors < 0) return ILQR_ERR_INVALID_ARGUMENT;
+  *bytes = slots_of(n_tensors) * sizeof(double);
+  return ILQR_OK;
+}
+
+int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors,
+                        int32_t norm_type, float* norm, float* tensor_norms, double* total, void* workspace,
+                        size_t workspace_bytes, cudaStream_t stream) {
+  const List l{grads, nullptr, numel, dtypes, n_tensors};
+  if (const int st = check_list(l, norm_type); st != ILQR_OK) return st;
+  if (norm == nullptr && tensor_norms == nullptr && total == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
+  if (n_tensors == 0) {
+    cudaError_t e = cudaSuccess;
+    if (norm != nullptr) e = cudaMemsetAsync(norm, 0, sizeof(float), stream);
+    if (e == cudaSuccess && total != nullptr) e = cudaMemsetAsync(total, 0, sizeof(double), stream);
+    return status_of(e);
+  }
+  if (workspace == nullptr || workspace_bytes < slots_of(n_tensors) * sizeof(double)) return ILQR_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 7u) return ILQR_ERR_MISALIGNED;
+  try {
+    const ilqr::GradNormOut o{norm, tensor_norms, total};
+    double* slots = static_cast<double*>(workspace);
+    const bool mx = norm_type == ILQR_NORM_MAX;
+    return n_tensors <= ilqr::GRAD_CAP_SHORT ? norm_impl<ilqr::GRAD_CAP_SHORT>(l, mx, o, slots, stream)
+                                             : norm_impl<ilqr::GRAD_CAP_LONG>(l, mx, o, slots, stream);
+  } catch (...) {
+    return ILQR_ERR_HOST_MEMORY;
+  }
+}
+
+int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtypes,
+                        int32_t n_tensors, int32_t norm_type, double max_norm, double eps, const double* total,
+                        float* norm, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (n_tensors > 0 && out == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
+  const List l{grads, out, numel, dtypes, n_tensors};
+  if (const int st = check_list(l, norm_type); st != ILQR_OK) return st;
+  if (!(max_norm >= 0.0) || !(eps >= 0.0) || std::isinf(eps)) return ILQR_ERR_INVALID_ARGUMENT;
+  if (total != nullptr && ((uintptr_t)total & 7u)) return ILQR_ERR_MISALIGNED;
+  if (workspace == nullptr || workspace_bytes < slots_of(n_tensors) * sizeof(double)) return ILQR_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 7u) return ILQR_ERR_MISALIGNED;
+  double* slots = static_cast<double*>(workspace);
+  const ilqr::GradScale s{max_norm, eps, norm_type == ILQR_NORM_MAX ? 1 : 0};
+  if (n_tensors == 0) {
+    if (norm == nullptr) return ILQR_OK;
+    if (total == nullptr) return status_of(cudaMemsetAsync(norm, 0, sizeof(float), stream));
+    const ilqr::GradNormOut o{norm, nullptr, nullptr};
+    return status_of(ilqr::launch_grad_join<ilqr::GRAD_CAP_SHORT>(nullptr, 0, nullptr, s.max_type != 0, total, 1, o,
+                                                                  true, stream));
+  }
+  try {
+    if (overlaps(l)) return ILQR_ERR_OVERLAP;
+    return n_tensors <= ilqr::GRAD_CAP_SHORT ? clip_impl<ilqr::GRAD_CAP_SHORT>(l, s, total, norm, slots, stream)
+                                             : clip_impl<ilqr::GRAD_CAP_LONG>(l, s, total, norm, slots, stream);
+  } catch (...) {
+    return ILQR_ERR_HOST_MEMORY;
+  }
+}
+
+}  // extern "C"
+
+namespace {
+
+// Where the slices of one tensor lie, in bytes.
+struct Rows {
+  uintptr_t base;
+  int64_t row, seg, len, n_seg, B;
+  uintptr_t lo() const { return base; }
+  uintptr_t hi() const { return base + (uintptr_t)((B - 1) * row + (n_seg - 1) * seg + len); }
+};
+
+// Whether no two of its values share memory: one of the two strides steps over
+// all that the other spans.
+bool apart(const Rows& r) {
+  if (r.row < 0 || r.seg < 0) return false;
+  const bool one_row = r.B == 1, one_seg = r.n_seg == 1;
+  if (!one_row && r.row < r.len) return false;
+  if (!one_seg && r.seg < r.len) return false;
+  if (one_row || one_seg) return true;
+  return r.row >= (r.n_seg - 1) * r.seg + r.len || r.seg >= (r.B - 1) * r.row + r.len;
+}
+
+// Whether two sets of slices share no memory. Spans that interleave are told
+// apart where both are single segments of rows with one stride (columns of
+// one packed array).
+bool disjoint(const Rows& a, const Rows& b) {
+  if (a.hi() <= b.lo() || b.hi() <= a.lo()) return true;
+  if (a.n_seg != 1 || b.n_seg != 1 || a.row != b.row || a.B == 1) return false;
+  const Rows& x = a.base <= b.base ? a : b;
+  const Rows& y = a.base <= b.base ? b : a;
+  const int64_t at = (int64_t)((y.base - x.base) % (uintptr_t)x.row);
+  return at >= x.len && at + y.len <= x.row;
+}
+
+bool same(const Rows& a, const Rows& b) {
+  return a.base == b.base && (a.B == 1 || a.row == b.row) && (a.n_seg == 1 || a.seg == b.seg);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, const int32_t* dtypes,
+                                 const int64_t* layout, int32_t n_tensors, int64_t B, double max_norm, double eps,
+                                 int32_t zero_nonfinite, float* norms, cudaStream_t stream) {
+  if (n_tensors < 1 || n_tensors > ILQR_MAX_ELEMENT_TENSORS || B < 0 || B > ILQR_MAX_BATCH)
+    return ILQR_ERR_INVALID_ARGUMENT;
+  if (grads == nullptr || out == nullptr || dtypes == nullptr || layout == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
+  if (!(max_norm >= 0.0) || !(eps >= 0.0) || std::isinf(eps)) return ILQR_ERR_INVALID_ARGUMENT;
+  if (B == 0) return ILQR_OK;
+  constexpr int64_t FAR = (int64_t)1 << 44;  // bytes: no address arithmetic below can wrap
+  ilqr::RowTable tab;
+  std::memset(&tab, 0, sizeof(tab));
+  Rows ins[ILQR_MAX_ELEMENT_TENSORS], outs[ILQR_MAX_ELEMENT_TENSORS];
+  int64_t row_bytes = 0;
+  for (int32_t i = 0; i < n_tensors; ++i) {
+    const int64_t* g = layout + 6 * i;
+    const int64_t n_seg = g[0], len = g[1];
+    if (dtypes[i] < ILQR_DTYPE_F32 || dtypes[i] > ILQR_DTYPE_BF16) return ILQR_ERR_INVALID_ARGUMENT;
+    if (n_seg < 0 || len < 0) return ILQR_ERR_INVALID_ARGUMENT;
+    if (n_seg == 0 || len == 0) continue;
+    const int64_t sz = size_of(dtypes[i]);
+    if (n_seg > INT32_MAX || len > INT32_MAX || n_seg * len > INT32_MAX) return ILQR_ERR_INVALID_ARGUMENT;
+    for (int k = 2; k < 6; ++k) {
+      const int64_t times = (k & 1) ? B : n_seg;  // [2] in_seg, [3] in_row, [4] out_seg, [5] out_row
+      if (magnitude(g[k]) > FAR / sz || (times > 1 && magnitude(g[k]) > FAR / sz / times))
+        return ILQR_ERR_INVALID_ARGUMENT;
+    }
+    if (grads[i] == nullptr || out[i] == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
+    const uintptr_t p = (uintptr_t)grads[i], q = (uintptr_t)out[i];
+    if ((p | q) & (uintptr_t)(sz - 1)) return ILQR_ERR_MISALIGNED;
+    const int k = tab.n++;
+    ins[k] = Rows{p, g[3] * sz, g[2] * sz, len * sz, n_seg, B};
+    outs[k] = Rows{q, g[5] * sz, g[4] * sz, len * sz, n_seg, B};
+    if (ins[k].row < 0 || ins[k].seg < 0) return ILQR_ERR_INVALID_ARGUMENT;
+    if (!apart(outs[k])) return ILQR_ERR_OVERLAP;
+    // the widest vector that divides every address and length
+    uintptr_t all = p | q | (uintptr_t)(len * sz) | 16u;
+    if (n_seg > 1) all |= (uintptr_t)ins[k].seg | (uintptr_t)outs[k].seg;
+    if (B > 1) all |= (uintptr_t)ins[k].row | (uintptr_t)outs[k].row;
+    const uint32_t vec = (uint32_t)(all & (~all + 1));
+    tab.t[k] = ilqr::RowTensor{static_cast<const char*>(grads[i]), static_cast<char*>(out[i]), ins[k].row, ins[k].seg,
+                               outs[k].row, outs[k].seg, (uint32_t)n_seg, (uint32_t)(len * sz / vec), vec,
+                               (uint32_t)dtypes[i]};
+    row_bytes += n_seg * len * sz;
+  }
+  for (int a = 0; a < tab.n; ++a)
+    for (int b = 0; b < tab.n; ++b) {
+      if (a != b && (!disjoint(outs[a], outs[b]) || !disjoint(outs[a], ins[b]))) return ILQR_ERR_OVERLAP;
+      if (a == b && !same(ins[a], outs[a]) && !disjoint(outs[a], ins[a])) return ILQR_ERR_OVERLAP;
+    }
+  // in place is told by the address alone in the kernel
+  tab.B = B;
+  tab.max_norm = max_norm;
+  tab.eps = eps;
+  tab.zero_nonfinite = zero_nonfinite != 0 ? 1 : 0;
+  tab.norms = norms;
+  return status_of(ilqr::launch_grad_rows(tab, row_bytes, stream));
+}
+
+}  // extern "C"

@@ -45,7 +45,9 @@ typedef enum {
   ILQR_ERR_WORKSPACE = 3,        /* workspace missing or too small */
   ILQR_ERR_CUDA = 4,             /* launch or driver-entry-point failure */
   ILQR_ERR_UNSUPPORTED_DEVICE = 5,
-  ILQR_ERR_NOALLOC_LIMIT = 6     /* problem needs more than the fixed no-allocation scratch */
+  ILQR_ERR_NOALLOC_LIMIT = 6,    /* problem needs more than the fixed no-allocation scratch */
+  ILQR_ERR_OVERLAP = 7,          /* an output shares memory with another tensor of the call */
+  ILQR_ERR_HOST_MEMORY = 8       /* host memory for the call's records could not be had */
 } ilqr_status_t;
 
 /* Per-element status bits written to elem_status[b] by ilqr_b200_solve_f32. */
@@ -468,6 +470,67 @@ int ilqr_b200_fastmpc_assembly_f32(
     const float* X, const float* U, const float* x_ref, const float* u_ref,
     int64_t B, int32_t T, float* grad_C, float* grad_c, float* grad_x0, float* grad_x_ref,
     float* grad_u_ref, float* grad_C_final, float* grad_c_final, cudaStream_t stream);
+
+/*
+ * Gradient norms and clipping: what a trainer does with gradients between its
+ * backward and its update (the reference's PPO update clips the policy's
+ * gradients to max_grad_norm, stable_baselines3/ppo/ppo.py:274-277). They take
+ * tensors of three types; the host arrays that describe the tensors are read
+ * during the call only.
+ */
+#define ILQR_DTYPE_F32 0
+#define ILQR_DTYPE_F16 1
+#define ILQR_DTYPE_BF16 2
+#define ILQR_NORM_L2 0  /* sqrt of the sum of squares */
+#define ILQR_NORM_MAX 1 /* largest magnitude */
+
+/* Device workspace (8-byte aligned) of ilqr_b200_grad_norm and
+ * ilqr_b200_grad_clip for a list of n_tensors. */
+int ilqr_b200_grad_workspace_size(int32_t n_tensors, size_t* bytes);
+
+/*
+ * Norm over all values of a list of tensors. HOST arrays of n_tensors: grads
+ * (device pointers, aligned to their type), numel, dtypes (ILQR_DTYPE_*). Each
+ * tensor is numel values without gaps, in any order. At most 2^40 values.
+ * Outputs (device, NULL to skip, one at least): norm [1], tensor_norms
+ * [n_tensors], total [1] (the sum of squares, or the largest magnitude, in 64
+ * bits: what several devices add up, or take the largest of). An empty list
+ * has norm 0. NaN values give NaN. A norm above the largest float shows as
+ * infinity in norm and tensor_norms (clipping goes by its 64-bit value).
+ */
+int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors,
+                        int32_t norm_type, float* norm, float* tensor_norms, double* total,
+                        void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
+ * out = c grads over a list, c = min(1, max_norm / (norm + eps)); max_norm =
+ * infinity leaves the values as they are, a NaN norm makes them NaN. out: HOST
+ * array of device pointers; out[i] may be grads[i] (in place), otherwise no
+ * output may share memory with any other tensor of the call (ILQR_ERR_OVERLAP).
+ * total: device, the sum of squares (largest magnitude) to clip by, or NULL
+ * for the list's own. norm (device, NULL to skip): the norm before clipping.
+ */
+int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtypes,
+                        int32_t n_tensors, int32_t norm_type, double max_norm, double eps, const double* total,
+                        float* norm, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
+ * The 2-norm form for each of B batch elements by itself: element b's gradient
+ * is its slices of n_tensors (1..8) tensors, norms[b] (device, NULL to skip)
+ * its norm, and its slices are scaled by min(1, max_norm / (norms[b] + eps)).
+ * zero_nonfinite: an element whose gradient holds an infinity or a NaN is set
+ * to zero instead (its norms[b] still shows it). layout: HOST array of six
+ * numbers for each tensor, in values: segments of an element, length of a
+ * segment, then strides of the input's segments, the input's elements, the
+ * output's segments and the output's elements. A batch-major [B, ...] tensor
+ * is {1, len, 0, len, 0, len}, a time-major [T, B, ...] one
+ * {T, len, B len, len, B len, len}. At most 2^31 - 1 values of an element in
+ * one tensor. Outputs as in ilqr_b200_grad_clip.
+ */
+#define ILQR_MAX_ELEMENT_TENSORS 8
+int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, const int32_t* dtypes,
+                                 const int64_t* layout, int32_t n_tensors, int64_t B, double max_norm, double eps,
+                                 int32_t zero_nonfinite, float* norms, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

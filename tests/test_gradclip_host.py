@@ -1,0 +1,166 @@
+"""CPU tests of the gradient norms and clipping: the C ABI's checks of its
+arguments (nothing is launched on a refused call) and the binding's."""
+
+import ctypes
+import math
+from array import array
+
+import pytest
+import torch
+
+import ilqr_native as nat
+
+A = 0x10000  # stands for a device address
+
+
+def _arr(code, *v):
+    return array(code, v)
+
+
+def _at(a):
+    return a.buffer_info()[0] if isinstance(a, array) else a
+
+
+def _norm(grads=(A, 2 * A), numel=(5, 7), dtypes=(0, 2), n=2, kind=0, norm=A, norms=None, total=None, ws=A,
+          ws_bytes=1 << 30):
+    g, s, t = _arr("Q", *grads), _arr("q", *numel), _arr("i", *dtypes)
+    return nat.lib().ilqr_b200_grad_norm(_at(g), _at(s), _at(t), n, kind, norm, norms, total, ws, ws_bytes, None)
+
+
+def _clip(grads=(A, 2 * A), out=(3 * A, 4 * A), numel=(5, 7), dtypes=(0, 0), n=2, kind=0, max_norm=1.0, eps=1e-6,
+          total=None, ws=A, ws_bytes=1 << 30):
+    g, o, s, t = _arr("Q", *grads), _arr("Q", *out), _arr("q", *numel), _arr("i", *dtypes)
+    return nat.lib().ilqr_b200_grad_clip(_at(g), _at(o), _at(s), _at(t), n, kind, max_norm, eps, total, None, ws,
+                                         ws_bytes, None)
+
+
+def _elements(grads=(A,), out=(2 * A,), dtypes=(0,), layout=((1, 10, 0, 10, 0, 10),), B=4, max_norm=1.0, eps=1e-6,
+              n=None):
+    g, o, t = _arr("Q", *grads), _arr("Q", *out), _arr("i", *dtypes)
+    lay = _arr("q", *[v for row in layout for v in row])
+    return nat.lib().ilqr_b200_grad_clip_elements(_at(g), _at(o), _at(t), _at(lay), len(grads) if n is None else n, B,
+                                                  max_norm, eps, 0, None, None)
+
+
+def test_workspace_size():
+    n = ctypes.c_size_t()
+    f = nat.lib().ilqr_b200_grad_workspace_size
+    sizes = []
+    for k in (0, 1, 60, 61, 1000, 1001, 5000):
+        assert f(k, ctypes.byref(n)) == 0 and n.value % 8 == 0
+        sizes.append(n.value)
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert f(-1, ctypes.byref(n)) == 1 and f(3, None) == 1
+
+
+def test_norm_refusals():
+    assert _norm(n=-1) == 1
+    assert _norm(kind=2) == 1
+    assert _norm(dtypes=(0, 3)) == 1 and _norm(dtypes=(-1, 0)) == 1
+    assert _norm(numel=(5, -1)) == 1
+    assert _norm(numel=(5, (1 << 40) + 1)) == 1
+    assert _norm(numel=(1 << 40, 1 << 40)) == 1
+    assert _norm(grads=(A, 0)) == 1
+    assert _norm(grads=(A + 2, A), dtypes=(0, 0)) == 2      # a float at an odd half
+    assert _norm(grads=(A, A + 1), dtypes=(0, 2)) == 2
+    assert _norm(norm=None) == 1                              # nothing to write
+    assert _norm(ws=None) == 3 and _norm(ws_bytes=8) == 3
+    assert _norm(ws=A + 4) == 2
+
+
+def test_clip_refusals():
+    assert _clip(kind=5) == 1
+    assert _clip(out=(A, 0)) == 1
+    for bad in (-1.0, math.nan):
+        assert _clip(max_norm=bad) == 1 and _clip(eps=bad) == 1
+    assert _clip(eps=math.inf) == 1
+    assert _clip(total=A + 4) == 2
+    assert _clip(out=(A + 2, 4 * A)) == 2
+    assert _clip(ws=None) == 3
+    # an output that another tensor of the call shares
+    assert _clip(out=(3 * A, 3 * A)) == 7
+    assert _clip(grads=(A, A), out=(A, A)) == 7                # the same tensor twice, in place
+    assert _clip(out=(A + 4, 4 * A)) == 7                      # its own input, shifted
+    assert _clip(out=(2 * A, 4 * A)) == 7                      # the other's input
+    assert _clip(out=(3 * A, 3 * A + 16), numel=(5, 7)) == 7   # 20 bytes, then 4 of them again
+    assert _clip(grads=(A, 2 * A), out=(A, 3 * A), numel=((2 * A - A) // 4 + 1, 7)) == 7
+
+
+def test_elements_refusals():
+    assert _elements(n=0) == 1 and _elements(grads=(A,) * 9, out=(A,) * 9, dtypes=(0,) * 9,
+                                             layout=((1, 1, 0, 1, 0, 1),) * 9) == 1
+    assert _elements(B=-1) == 1 and _elements(B=1 << 31) == 1
+    assert _elements(B=0) == 0
+    assert _elements(dtypes=(3,)) == 1
+    assert _elements(max_norm=-1.0) == 1 and _elements(max_norm=math.nan) == 1 and _elements(eps=math.inf) == 1
+    assert _elements(grads=(0,)) == 1 and _elements(out=(0,)) == 1
+    assert _elements(layout=((-1, 10, 0, 10, 0, 10),)) == 1
+    assert _elements(layout=((2, (1 << 30) + 1, 0, 10, 0, 10),)) == 1
+    assert _elements(layout=((1, 10, 0, 1 << 60, 0, 10),)) == 1    # no byte offset wraps
+    assert _elements(layout=((1, 10, 0, -10, 0, 10),)) == 1
+    assert _elements(grads=(A + 2,)) == 2 and _elements(out=(2 * A + 1,)) == 2
+    assert _elements(layout=((1, 10, 0, 10, 0, 9),)) == 7           # output slices share a value
+    assert _elements(layout=((1, 10, 0, 10, 0, 0),)) == 7           # every element into one slice
+    assert _elements(layout=((3, 10, 40, 10, 39, 10),)) == 7        # segments into one another
+    assert _elements(out=(A + 40,)) == 7                            # its own input, one element on
+    two = dict(dtypes=(0, 0), B=4)
+    assert _elements(grads=(A, 2 * A), out=(3 * A, 3 * A + 4), layout=((1, 10, 0, 30, 0, 30),) * 2, **two) == 7
+    assert _elements(grads=(A, A), out=(A, A), layout=((1, 10, 0, 10, 0, 10),) * 2, **two) == 7
+
+
+def test_binding_refusals_without_gpu():
+    x = torch.zeros(3)
+    with pytest.raises(TypeError):
+        nat.grad_norm(x)
+    with pytest.raises(TypeError):
+        nat.grad_norm([3])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.grad_norm([x])
+    with pytest.raises(RuntimeError, match="empty"):
+        nat.grad_norm([])
+    with pytest.raises(ValueError, match="norm_type"):
+        nat.grad_norm([x], norm_type=1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        nat.clip_grad_norm([x], -1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        nat.clip_grad_norm([x], math.nan)
+    with pytest.raises(ValueError, match="eps"):
+        nat.clip_grad_norm([x], 1.0, eps=-1e-6)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.clip_grad_norm([x], 1.0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.clip_grad_elements([x], 1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        nat.clip_grad_elements([x], math.nan)
+
+
+def test_how_slices_lie_in_memory():
+    """Batch-major, time-major, permuted and strided gradients as segments."""
+    T, B = 3, 5
+    seg = nat._segments
+    C = torch.empty(B, T, 14, 14)
+    assert seg(C, C, 0) == (1, T * 196, 0, T * 196, 0, T * 196)
+    Ct = torch.empty(T, B, 14, 14)
+    assert seg(Ct, Ct, 1) == (T, 196, B * 196, 196, B * 196, 196)
+    v = Ct.permute(1, 0, 2, 3)
+    assert seg(v, v, 0) == (T, 196, B * 196, 196, B * 196, 196)
+    assert seg(v, C, 0) == (T, 196, B * 196, 196, 196, T * 196)
+    packed = torch.empty(B, 30)
+    assert seg(packed[:, 10:24], packed[:, 10:24], 0) == (1, 14, 0, 30, 0, 30)
+    assert seg(torch.empty(B), torch.empty(B), 0)[:2] == (1, 1)
+    last = torch.empty(7, B)
+    assert seg(last, last, 1) == (7, 1, B, 1, B, 1)
+    wide = torch.empty(B, 6, 8, 10)[:, ::2, ::2, :]
+    assert seg(wide, wide, 0) is None
+    one = torch.empty(1).expand(B, 4)
+    assert seg(one, torch.empty(B, 4), 0) == (4, 1, 0, 0, 1, 4)
+    assert seg(torch.empty(B, 0, 3), torch.empty(B, 0, 3), 0)[0:2].count(0) == 1
+
+
+def test_which_tensors_have_gaps():
+    x = torch.empty(4, 6, 5)
+    assert nat._without_gaps(x) and nat._without_gaps(x.permute(2, 0, 1)) and nat._without_gaps(x[1:3])
+    assert nat._without_gaps(torch.empty(())) and nat._without_gaps(torch.empty(0, 3))
+    assert not nat._without_gaps(x[:, 1:]) and not nat._without_gaps(torch.empty(3).expand(2, 3))
+    assert nat._one_to_a_place(x[:, 1:]) and not nat._one_to_a_place(torch.empty(3).expand(2, 3))
+    assert not nat._one_to_a_place(torch.empty(9).as_strided((4, 3), (2, 1)))
