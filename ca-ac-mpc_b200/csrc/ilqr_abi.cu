@@ -43,9 +43,19 @@ int encode_cost_map(CUtensorMap* tm, const float* base, int64_t B, int32_t T, bo
   const cuuint32_t box[3] = {(cuuint32_t)ilqr::CBLK, 1u, (cuuint32_t)ilqr::EPW};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
   std::memset(tm, 0, sizeof(*tm));
-  const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto encode = [&] {
+    return fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread whose first CUDA call this is (autograd's, when no torch kernel
+    // ran on it before) has no context yet: a driver call does not make one
+    // current as runtime calls do.
+    int device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = encode();
+  }
   return r == CUDA_SUCCESS ? ILQR_OK : ILQR_ERR_CUDA;
 }
 
