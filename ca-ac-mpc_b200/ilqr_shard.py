@@ -5,15 +5,20 @@ contiguous slice [lo, hi) of the batch with no communication. After the
 solve, the results the caller consumes are gathered over torch.distributed
 (NCCL on GPUs, gloo on CPU): the first controls U[:, 0, :] (the actions the
 policy steps with) and, after the backward, the gradients (dL/dx0 by
-default; dL/dc or dL/dC on request). The reference has no multi-GPU path; its
+default; dL/dc or dL/dC on request), or clipped by their norm over all ranks
+where they are. The reference has no multi-GPU path; its
 caller solves the whole batch in one process
 (acmpc_public-master/training_modules/mlp_mpc_policy_diffmpc.py:324-399).
 """
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.distributed as dist
+
+import ilqr_native as _nat
 
 
 def shard_bounds(B: int, rank: int, world: int):
@@ -86,3 +91,31 @@ def gather_gradients(grads: dict, B: int, keys=("x0",), group=None) -> dict:
     tensors: dL/dx0 [B, 10] by default, "c" [B, T, 14] or "C" [B, T, 14, 14]
     when the consumer lives on rank 0."""
     return {k: gather_rows(grads[k], B, group) for k in keys}
+
+
+def grad_norm_total(grads, norm_type: float = 2.0, group=None) -> torch.Tensor:
+    """ilqr_native.grad_norm_total over the gradients of every rank: the sum
+    of squares (norm_type inf: the largest magnitude) of all shards, a 0-d
+    float64 tensor that is the same on every rank."""
+    total = _nat.grad_norm_total(grads, norm_type)
+    if math.isinf(float(norm_type)):
+        # a maximum across ranks may pass over a NaN: it travels beside it
+        bad = total.isnan()
+        pair = torch.stack([torch.where(bad, torch.zeros_like(total), total), bad.to(total.dtype)])
+        dist.all_reduce(pair, op=dist.ReduceOp.MAX, group=group)
+        return torch.where(pair[1] > 0, torch.full_like(total, math.nan), pair[0])
+    dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
+    return total
+
+
+def clip_gradients(grads: dict, max_norm: float, norm_type: float = 2.0, group=None) -> torch.Tensor:
+    """Clip the gradients of a rank's backward (the dict ilqr_native.backward
+    returns) in place by the norm over the whole batch, whose elements lie on
+    the group's ranks: one all-reduce of a scalar, and every rank scales its
+    shard by the same factor. Returns that norm. Every rank of the group calls
+    it, one with an empty shard too. (Gradients that every rank holds alike,
+    those of a replicated network, have no part here: they would be counted
+    once for each rank; a rank clips them by itself.)"""
+    held = list(grads.values())
+    total = grad_norm_total(held, norm_type, group)
+    return _nat.clip_grad_norm(held, max_norm, norm_type=norm_type, total=total, out=held)[1]

@@ -150,6 +150,59 @@ def _f32(t):
     return None if t is None else t.to(torch.float32).contiguous()
 
 
+class GradClip:
+    """How FastMPC's backward clips the gradients it returns, and the norms it
+    found. mode "element": each batch element's gradient (its slices of all
+    the returned tensors) by its own norm; "batch": all of them together."""
+
+    def __init__(self, max_norm: float, mode: str = "element", zero_nonfinite: bool = False):
+        if mode not in ("element", "batch"):
+            raise ValueError(f"grad_clip must be 'element' or 'batch', not {mode!r}")
+        if zero_nonfinite and mode != "element":
+            raise ValueError("zero_nonfinite_grad sets single elements to zero: it needs grad_clip='element'")
+        if not float(max_norm) >= 0.0:
+            raise ValueError(f"max_grad_norm must not be negative or NaN, got {max_norm}")
+        self.max_norm = float(max_norm)
+        self.mode = mode
+        self.zero_nonfinite = bool(zero_nonfinite)
+        self.norms: Optional[Tensor] = None  # [B] ("element") or a scalar ("batch"), on the device
+
+    def __call__(self, grads, batch_dims, out=None):
+        if self.mode == "element":
+            got, self.norms = _nat.clip_grad_elements(grads, self.max_norm, batch_dims=batch_dims,
+                                                      zero_nonfinite=self.zero_nonfinite, out=out)
+        else:
+            got, self.norms = _nat.clip_grad_norm(grads, self.max_norm, out=out)
+        return got
+
+    def in_place(self, grads: dict, time_major: bool):
+        """Clip a backward's dict of new gradients (C and c time-major or not)."""
+        held = list(grads.values())
+        self(held, [int(time_major and k in ("C", "c")) for k in grads], out=held)
+
+
+class GradClipFunction(torch.autograd.Function):
+    """The inputs as they are; their gradients, batch first, clipped on the
+    way back. For inputs whose gradients come out of several operations, where
+    there is no one backward to clip in."""
+
+    @staticmethod
+    def forward(ctx, clip, *inputs):
+        ctx.clip = clip
+        ctx.set_materialize_grads(False)
+        return tuple(x.view_as(x) for x in inputs)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[1 + i]]
+        out = list(grads)
+        if at:
+            # other consumers may hold the incoming tensors: into new ones
+            for i, g in zip(at, ctx.clip([grads[i] for i in at], 0)):
+                out[i] = g
+        return (None, *out)
+
+
 class DroneMPCFunction(torch.autograd.Function):
     """Differentiable batched iLQR solve.
 
@@ -179,6 +232,7 @@ class DroneMPCFunction(torch.autograd.Function):
                               _f32(x_ref) if x_ref is not None else None, out["tight"])
         ctx.dt = float(solver_cfg["dt"])
         ctx.reg_eps = float(solver_cfg.get("reg_eps", solver_cfg["eps"]))
+        ctx.grad_clip = solver_cfg.get("grad_clip")
         return X, U
 
     @staticmethod
@@ -194,6 +248,8 @@ class DroneMPCFunction(torch.autograd.Function):
         bwd = _nat.rotor13_backward if ctx.r13 else _nat.backward
         g = bwd(X, U, C_bt, gX, gU, C_final=C_final, x_ref=x_ref, tight=tight,
                 dt=ctx.dt, reg_eps=ctx.reg_eps, need=want, time_major=ctx.time_major)
+        if ctx.grad_clip is not None:
+            ctx.grad_clip.in_place(g, ctx.time_major)
         return tuple(g.get(nm) for nm in names) + (None,)
 
 
@@ -264,6 +320,7 @@ class SigmoidMPCFunction(torch.autograd.Function):
         ctx.spec = spec
         ctx.dt = float(solver_cfg["dt"])
         ctx.reg_eps = float(solver_cfg.get("reg_eps", solver_cfg["eps"]))
+        ctx.grad_clip = solver_cfg.get("grad_clip")
         return X, U
 
     @staticmethod
@@ -277,6 +334,8 @@ class SigmoidMPCFunction(torch.autograd.Function):
         gU = torch.zeros_like(U) if grad_U is None else grad_U.to(torch.float32).contiguous()
         g = _nat.backward_sigmoid(X, U, sc, gX, gU, ctx.spec, tight=tight, dt=ctx.dt,
                                   reg_eps=ctx.reg_eps, need=want)
+        if ctx.grad_clip is not None:
+            ctx.grad_clip.in_place(g, False)
         return g.get("x0"), g.get("sigmoid_cost"), None
 
 
@@ -299,6 +358,7 @@ class FastMPCNumericsFunction(torch.autograd.Function):
         ctx.save_for_backward(X, U, out["X_lin"], out["U_lin"], C32, out["tight"] if bounded else None)
         ctx.dt = float(solver_cfg["dt"])
         ctx.reg_eps = float(solver_cfg.get("reg_eps", solver_cfg["eps"]))
+        ctx.grad_clip = solver_cfg.get("grad_clip")
         return X, U
 
     @staticmethod
@@ -311,6 +371,8 @@ class FastMPCNumericsFunction(torch.autograd.Function):
         gU = torch.zeros_like(U) if grad_U is None else grad_U.to(torch.float32).contiguous()
         g = _nat.fastmpc_backward(X, U, X_lin, U_lin, C32, gX, gU, tight=tight, dt=ctx.dt, reg_eps=ctx.reg_eps,
                                   need=want, time_major=True)
+        if ctx.grad_clip is not None:
+            ctx.grad_clip.in_place(g, True)
         return g.get("x0"), g.get("C"), g.get("c"), None
 
 
@@ -325,6 +387,13 @@ class FastMPC(nn.Module):
     numerics: "diffmpc" (default) or "fastmpc" (the reference FastMPC build's
     own numerics; 10-state model; a SigmoidQuadCost is turned into the dense
     costs the policy would build; ACMPC_FASTMPC_NUMERICS sets the default).
+    max_grad_norm clips the gradients that the backward returns, which are
+    those of x_init (float32, batch first) and of the costs (time-major, before
+    they are summed over what was broadcast; a SigmoidQuadCost's: of its
+    sigmoid output) as far as they are asked for: grad_clip="element" each
+    batch element's by its own norm, "batch" all of them together;
+    zero_nonfinite_grad sets elements whose gradient holds an infinity or a NaN
+    to zero. The norms before clipping are in grad_norms after the backward.
     """
 
     def __init__(self, n_state: int, n_ctrl: int, T: int, u_lower: Optional[Tensor] = None,
@@ -334,8 +403,12 @@ class FastMPC(nn.Module):
                  max_linesearch_iter: int = 10, grad_method: GradMethods = GradMethods.ANALYTIC,
                  eps: float = 1e-6, n_batch: Optional[int] = None, backprop: bool = True,
                  slew_rate_penalty: Optional[float] = None, prev_ctrl: Optional[Tensor] = None,
-                 alphas=None, numerics: Optional[str] = None, **kwargs):
+                 alphas=None, numerics: Optional[str] = None, max_grad_norm: Optional[float] = None,
+                 grad_clip: str = "element", zero_nonfinite_grad: bool = False, **kwargs):
         super().__init__()
+        self.grad_clip = (GradClip(float("inf") if max_grad_norm is None else max_grad_norm, grad_clip,
+                                   zero_nonfinite_grad)
+                          if max_grad_norm is not None or zero_nonfinite_grad else None)
         numerics = (numerics or os.environ.get("ACMPC_FASTMPC_NUMERICS", "diffmpc")).strip().lower()
         if numerics not in ("diffmpc", "fastmpc"):
             raise ValueError(f"numerics must be 'diffmpc' or 'fastmpc', not {numerics!r}")
@@ -360,6 +433,11 @@ class FastMPC(nn.Module):
         self._dt = 0.02
         self._bounds_key = None
         self._bounds = (None, None)
+
+    @property
+    def grad_norms(self) -> Optional[Tensor]:
+        """The norms that the last backward clipped by, before clipping."""
+        return None if self.grad_clip is None else self.grad_clip.norms
 
     def _get_ext(self):
         if self._ext is None:
@@ -398,19 +476,25 @@ class FastMPC(nn.Module):
         r13 = nx == _nat.NX13
         if sigm and r13:
             raise ValueError("SigmoidQuadCost builds the 10-state policy's costs; use QuadCost with n_state=13")
+        x0 = x_init.float().contiguous()
+        grad_clip = self.grad_clip
         if sigm and self.numerics == "fastmpc":
             # the FastMPC kernels read dense costs: build the policy's C, c on
             # the device (autograd carries the gradient back to the sigmoid output)
-            C_tb, c_tb = _sigmoid_to_dense_tm(cost.sigmoid_cost.to(torch.float32), T, cost.spec())
+            sc = cost.sigmoid_cost.to(torch.float32)
+            if grad_clip is not None and torch.is_grad_enabled() and self.backprop:
+                x0, sc = GradClipFunction.apply(grad_clip, x0, sc)
+                grad_clip = None
+            C_tb, c_tb = _sigmoid_to_dense_tm(sc, T, cost.spec())
             sigm = False
         elif not sigm:
             C_tb, c_tb = _normalize_cost_tm(cost.C, cost.c, B, T, n, device, dtype)
         u_min, u_max = self._get_bounds(device, dtype)
         U_init = _normalize_init(self.u_init, B, T, nu, device, dtype, nx)
-        x0 = x_init.float().contiguous()
         cfg = {"U_init": U_init, "u_min": u_min, "u_max": u_max, "dt": float(dt),
                "lqr_iter": self.lqr_iter, "eps": self.eps, "converge_tol": 1e-6,
-               "reg_eps": self.eps, "nx": nx, "nu": nu, "alphas": self._alphas(), "time_major": True}
+               "reg_eps": self.eps, "nx": nx, "nu": nu, "alphas": self._alphas(), "time_major": True,
+               "grad_clip": grad_clip}
         if sigm:
             cfg["sigmoid_spec"] = cost.spec()
             if torch.is_grad_enabled() and self.backprop:

@@ -18,7 +18,7 @@ reference loop's on the same solver.
 from __future__ import annotations
 
 import os
-from typing import Optional
+from typing import Iterable, Optional, Union
 
 import torch
 from torch import Tensor
@@ -37,12 +37,15 @@ class PolicyMPC:
     Constants follow DroneDx (drone.py:166-203): mass, thrust_max per rotor,
     omega_max; the control box is [4 thrust_min, -omega_max] ..
     [4 thrust_max, omega_max] (mlp_mpc_policy_diffmpc.py:166-177). numerics:
-    as FastMPC's ("diffmpc" by default, or "fastmpc")."""
+    as FastMPC's ("diffmpc" by default, or "fastmpc"). max_grad_norm,
+    grad_clip, zero_nonfinite_grad: FastMPC's clipping of the gradients that
+    reach the policy network (its norms: solver.grad_norms)."""
 
     def __init__(self, T: int, dt: float, lqr_iter: Optional[int] = None, eps: float = 0.1,
                  alphas=None, mass: float = 0.752, thrust_min: float = 0.0, thrust_max: float = 8.5,
                  omega_max=(10.0, 10.0, 4.0), grad_mode: str = "diff", chunk: Optional[int] = None,
-                 device=None, numerics: Optional[str] = None):
+                 device=None, numerics: Optional[str] = None, max_grad_norm: Optional[float] = None,
+                 grad_clip: str = "element", zero_nonfinite_grad: bool = False):
         self.T = int(T)
         self.dt = float(dt)
         self.lqr_iter = int(os.environ.get("ACMPC_MPC_MAX_ITER", "1")) if lqr_iter is None else int(lqr_iter)
@@ -58,7 +61,9 @@ class PolicyMPC:
         hi = torch.tensor([4.0 * thrust_max, omega_max[0], omega_max[1], omega_max[2]], device=self.device)
         self.solver = mpc_compat.FastMPC(10, 4, self.T, u_lower=lo.view(1, 1, 4).expand(self.T, 1, 4),
                                          u_upper=hi.view(1, 1, 4).expand(self.T, 1, 4),
-                                         lqr_iter=self.lqr_iter, eps=self.eps, alphas=alphas, numerics=numerics)
+                                         lqr_iter=self.lqr_iter, eps=self.eps, alphas=alphas, numerics=numerics,
+                                         max_grad_norm=max_grad_norm, grad_clip=grad_clip,
+                                         zero_nonfinite_grad=zero_nonfinite_grad)
         self._dx = type("Dx", (), {"dt": self.dt})()
         self.u_prev: Optional[Tensor] = None
         self.predictions: Optional[Tensor] = None
@@ -106,4 +111,37 @@ class PolicyMPC:
         return torch.cat((thrust_normalized.unsqueeze(1), omegas_normalized), dim=1)
 
 
-__all__ = ["PolicyMPC"]
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> Tensor:
+    """Clip the gradients of the policy's parameters in place by their norm
+    together, as the update does between its backward and the optimiser's step
+    (th.nn.utils.clip_grad_norm_(policy.parameters(), max_grad_norm),
+    stable_baselines3/ppo/ppo.py:274-277): the same arguments and result, the
+    norm before clipping as a device scalar. Parameters without a gradient are
+    passed over; parameters on several devices are clipped by their joint
+    norm. norm_type: 2 or inf. Nothing reads back to the host unless
+    error_if_nonfinite asks for it."""
+    params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    lists = {}
+    for g in grads:
+        lists.setdefault(g.device, []).append(g)
+    total = None
+    if len(lists) > 1 or error_if_nonfinite:
+        first = grads[0].device
+        each = torch.stack([_nat.grad_norm_total(held, norm_type).to(first) for held in lists.values()])
+        total = each.sum() if float(norm_type) == 2.0 else each.max()
+        if error_if_nonfinite and not torch.isfinite(total):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, "
+                               "so it cannot be clipped.")
+    norm = None
+    for device, held in lists.items():
+        _, n = _nat.clip_grad_norm(held, max_norm, norm_type=norm_type, out=held,
+                                   total=None if total is None else total.to(device))
+        norm = n if norm is None else norm
+    return norm
+
+
+__all__ = ["PolicyMPC", "clip_grad_norm_"]

@@ -164,3 +164,103 @@ def test_which_tensors_have_gaps():
     assert not nat._without_gaps(x[:, 1:]) and not nat._without_gaps(torch.empty(3).expand(2, 3))
     assert nat._one_to_a_place(x[:, 1:]) and not nat._one_to_a_place(torch.empty(3).expand(2, 3))
     assert not nat._one_to_a_place(torch.empty(9).as_strided((4, 3), (2, 1)))
+
+
+# ---- the paths' host logic ---------------------------------------------------
+
+def test_operator_options_without_gpu():
+    import mpc_compat
+    m = mpc_compat.FastMPC(10, 4, 3)
+    assert m.grad_clip is None and m.grad_norms is None
+    m = mpc_compat.FastMPC(10, 4, 3, max_grad_norm=0.5)
+    assert m.grad_clip.mode == "element" and m.grad_clip.max_norm == 0.5 and m.grad_norms is None
+    m = mpc_compat.FastMPC(13, 4, 3, zero_nonfinite_grad=True)
+    assert m.grad_clip.max_norm == math.inf and m.grad_clip.zero_nonfinite
+    for bad in (dict(max_grad_norm=-1.0), dict(max_grad_norm=math.nan), dict(max_grad_norm=1.0, grad_clip="row"),
+                dict(max_grad_norm=1.0, grad_clip="batch", zero_nonfinite_grad=True)):
+        with pytest.raises(ValueError):
+            mpc_compat.FastMPC(10, 4, 3, **bad)
+
+
+def _plain(nat_module):
+    """Plain CPU stands-in for the two calls that the sharded clipping makes."""
+    def total(grads, norm_type=2.0):
+        flat = torch.cat([g.reshape(-1).double() for g in grads])
+        if norm_type == 2.0:
+            return flat.square().sum()
+        return flat.abs().max() if flat.numel() else torch.zeros((), dtype=torch.float64)
+
+    def clip(grads, max_norm, norm_type=2.0, total=None, out=None):
+        norm = total.sqrt() if norm_type == 2.0 else total
+        for g, o in zip(grads, out):
+            o.copy_(g * (max_norm / (norm + 1e-6)).clamp(max=1.0))
+        return out, norm.float()
+    nat_module.grad_norm_total, nat_module.clip_grad_norm = total, clip
+
+
+def _worker(rank, world, port, q):
+    import os
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path[:0] = [root, os.path.join(root, "ca-ac-mpc_b200")]
+    import torch.distributed as dist
+    import ilqr_native
+    import ilqr_shard as sh
+    _plain(ilqr_native)
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        said = []
+        for B, p, bad in ((7, 2.0, None), (7, math.inf, None), (1, 2.0, None), (7, math.inf, 6), (7, 2.0, 6)):
+            x0, c = _whole(B, bad)
+            lo, hi = sh.shard_bounds(B, rank, world)
+            g = {"x0": x0[lo:hi].clone(), "c": c[lo:hi].clone()}
+            n = sh.clip_gradients(g, 0.5, norm_type=p)
+            full = sh.gather_gradients(g, B, keys=("x0", "c"))
+            said.append((float(n), full["x0"].numpy(), full["c"].numpy()))
+        q.put((rank, said))
+    finally:
+        dist.destroy_process_group()
+
+
+def _whole(B, bad):
+    gen = torch.Generator().manual_seed(B)
+    x0, c = torch.randn(B, 10, generator=gen), torch.randn(B, 4, 14, generator=gen)
+    if bad is not None:
+        c[bad, 1, 2] = math.nan
+    return x0, c
+
+
+def test_sharded_clipping_over_two_ranks():
+    """Each rank scales by the norm of the whole batch; an empty shard takes
+    part, and a NaN on one rank reaches the other whatever the norm."""
+    import socket
+
+    import numpy as np
+    import torch.multiprocessing as mp
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=300) for _ in procs)
+    for p in procs:
+        p.join(timeout=120)
+        assert p.exitcode == 0
+    for k, (B, p, bad) in enumerate(((7, 2.0, None), (7, math.inf, None), (1, 2.0, None), (7, math.inf, 6),
+                                     (7, 2.0, 6))):
+        x0, c = _whole(B, bad)
+        flat = torch.cat([x0.reshape(-1), c.reshape(-1)]).double()
+        norm = float(flat.square().sum().sqrt()) if p == 2.0 else float(flat.abs().max())
+        for rank in range(2):
+            n, gx, gc = got[rank][k]
+            if bad is not None:
+                assert math.isnan(n) and np.isnan(gx).all() and np.isnan(gc).all()
+                continue
+            assert abs(n - norm) <= 2.0**-23 * norm
+            scale = min(1.0, 0.5 / (norm + 1e-6))
+            assert np.allclose(gx, x0.numpy() * scale, rtol=1e-6) and np.allclose(gc, c.numpy() * scale, rtol=1e-6)
