@@ -6,8 +6,10 @@ Compiles every .cu file in this directory with nvcc for sm_100a
 (-gencode arch=compute_100a,code=sm_100a, -lineinfo, -fmad=false so the model
 arithmetic rounds like the reference's elementwise torch ops; FILE_FLAGS adds
 per-file options) and links them
-into ca-ac-mpc_b200/libilqr_b200.so. Objects are rebuilt only when a source or
-header is newer than the object (make-style), in parallel.
+into ca-ac-mpc_b200/libilqr_b200.so, then the torch binding of the calls that
+take lists of tensors (binding/ilqr_torch.cpp) with g++ into
+ca-ac-mpc_b200/ilqr_torch.so, a Python module. Objects are rebuilt only when a
+source or header is newer than the object (make-style), in parallel.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -26,6 +29,8 @@ OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 LIB = os.path.join(PKG, "libilqr_b200.so")
 PROBE_LIB = os.path.join(PKG, "libilqr_probe.so")
 PROBE_SRC = os.path.join(HERE, "probe", "fma_probe.cu")
+BINDING_SRC = os.path.join(HERE, "binding", "ilqr_torch.cpp")
+BINDING = os.path.join(PKG, "ilqr_torch.so")
 NVCC = os.environ.get("NVCC", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-fmad=false", "-Xcompiler", "-fPIC,-O2",
@@ -42,6 +47,27 @@ def _newer(src_files, target):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(s) > t for s in src_files)
+
+
+def build_binding() -> str:
+    """The torch binding, against the torch that is importable here and the
+    C-ABI library beside it."""
+    import torch
+    at = os.path.dirname(torch.__file__)
+    public = os.path.join(ROOT, "include", "ilqr_b200.h")
+    # g++ as nvcc takes it (torch and this module share one libstdc++)
+    if _newer([BINDING_SRC, public, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
+        inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
+               sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+        cmd = ["g++", "-std=c++20", "-O2", "-fPIC", "-shared",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc],
+               BINDING_SRC, "-o", BINDING, f"-L{os.path.join(at, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+               "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{PKG}", "-l:libilqr_b200.so", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("torch binding build failed:\n" + r.stdout + r.stderr)
+    return BINDING
 
 
 def build(verbose: bool = False) -> str:
@@ -80,6 +106,7 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(link, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
+    build_binding()
     # FP32 FMA throughput probe used by the benchmark's roofline (separate
     # library: measurement only).
     if _newer([PROBE_SRC], PROBE_LIB):

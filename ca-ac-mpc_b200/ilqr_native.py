@@ -11,12 +11,11 @@ point requires CUDA tensors.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import importlib.util
 import math
 import os
 import threading
-from array import array
 from typing import Optional, Sequence
 
 import torch
@@ -962,84 +961,44 @@ def fastmpc_assembly(K, k, v0, A, Bm, X, U, x_ref=None, u_ref=None, compute_xref
 
 
 # ---- gradient norms and clipping -------------------------------------------
+#
+# Lists of up to thousands of tensors: the binding that reads them is native
+# too (csrc/binding/ilqr_torch.cpp, built beside the library).
 
-_GRAD_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_NORM_TYPES = {2.0: 0, math.inf: 1}
+BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "ilqr_torch.so")
 MAX_ELEMENT_TENSORS = 8
-_grad_ws_sizes = {}
+_binding_module = None
 
 
-def _grad_workspace_bytes(n: int) -> int:
-    got = _grad_ws_sizes.get(n)
-    if got is None:
-        b = ctypes.c_size_t(0)
-        _check(lib().ilqr_b200_grad_workspace_size(n, ctypes.byref(b)), "workspace query")
-        got = _grad_ws_sizes[n] = int(b.value)
-    return got
+def _binding():
+    """The native binding (loaded once). Raises if it has not been built."""
+    global _binding_module
+    if _binding_module is None:
+        lib()
+        with _lib_lock:
+            if _binding_module is None:
+                if not os.path.exists(BINDING_PATH):
+                    raise RuntimeError(f"{BINDING_PATH} is missing: build it with "
+                                       "`python ca-ac-mpc_b200/csrc/build.py` (or __graft_entry__.build())")
+                spec = importlib.util.spec_from_file_location("ilqr_torch", BINDING_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _binding_module = module
+    return _binding_module
 
 
-def _on(device: torch.device):
-    """Launches go to the current device: make that the tensors' own."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _grad_list(grads, name):
-    """The tensors of a list as a list, checked; and their device."""
-    if isinstance(grads, torch.Tensor):
+def _as_list(tensors, name):
+    if isinstance(tensors, torch.Tensor):
         raise TypeError(f"{name} must be a sequence of tensors, not one tensor")
-    grads = list(grads)
-    dev = None
-    for g in grads:
-        if not isinstance(g, torch.Tensor):
-            raise TypeError(f"{name} must hold tensors, not {type(g).__name__}")
-        if not g.is_cuda:
-            raise RuntimeError(f"{name} must hold CUDA tensors (no CPU path)")
-        if g.dtype not in _GRAD_DTYPES:
-            raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {g.dtype}")
-        if g.layout is not torch.strided:
-            raise RuntimeError(f"{name} must be dense tensors, got {g.layout}")
-        if dev is None:
-            dev = g.device
-        elif g.device != dev:
-            raise RuntimeError(f"{name} must be on one device, got {dev} and {g.device}")
-    return grads, dev
-
-
-def _without_gaps(t: torch.Tensor) -> bool:
-    """Whether t's values fill one run of memory, each in a place of its own."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _one_to_a_place(t: torch.Tensor) -> bool:
-    """Whether each of t's values has a place of its own: every stride steps
-    over all that the smaller ones span."""
-    span = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride < span:
-            return False
-        span = stride * (size - 1) + span
-    return True
-
-
-def _gathered(t: torch.Tensor) -> torch.Tensor:
-    """t's values in a new contiguous tensor."""
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return tensors if type(tensors) is list else list(tensors)
 
 
 def _norm_code(norm_type) -> int:
-    code = _NORM_TYPES.get(float(norm_type))
-    if code is None:
-        raise ValueError(f"norm_type must be 2 or inf, not {norm_type!r}")
-    return code
+    if norm_type == 2:
+        return 0
+    if norm_type == math.inf:
+        return 1
+    raise ValueError(f"norm_type must be 2 or inf, not {norm_type!r}")
 
 
 def _bound(max_norm, eps):
@@ -1051,83 +1010,22 @@ def _bound(max_norm, eps):
     return max_norm, eps
 
 
-def _arrays(tensors):
-    return (array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
-            array("i", [_GRAD_DTYPES[t.dtype] for t in tensors]))
-
-
-def _at(a):
-    return a.buffer_info()[0]
-
-
-def _grad_norm(grads, norm_type, want):
-    """(outputs named in `want`) for the norm over a list of gradients."""
-    code = _norm_code(norm_type)
-    grads, dev = _grad_list(grads, "grads")
-    if not grads:
-        raise RuntimeError("grads is empty: there is no device to put its norm on")
-    L = lib()
-    with _on(dev):
-        _device_ok(dev)
-        # values with gaps, or several to a place, are gathered first
-        use = [g if _without_gaps(g) else g.contiguous() for g in grads]
-        n = len(use)
-        shapes = {"norm": ((), torch.float32), "norms": ((n,), torch.float32), "total": ((), torch.float64)}
-        out = {k: torch.empty(shapes[k][0], dtype=shapes[k][1], device=dev) for k in want}
-        nbytes = _grad_workspace_bytes(n)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        ptrs, sizes, types = _arrays(use)
-        st = L.ilqr_b200_grad_norm(_at(ptrs), _at(sizes), _at(types), n, code, _ptr(out.get("norm")),
-                                   _ptr(out.get("norms")), _ptr(out.get("total")), ws.data_ptr(), nbytes, _stream(dev))
-    _check(st, "ilqr_b200_grad_norm")
-    return [out[k] for k in want]
-
-
 def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False):
     """Norm over all values of a sequence of gradients (float32, float16 or
     bfloat16, mixed as they come, any strides), a 0-d float32 tensor on their
     device; with per_tensor also each tensor's own norm, [n]. norm_type 2 or
     inf. Nothing is read back to the host."""
-    got = _grad_norm(grads, norm_type, ("norm", "norms") if per_tensor else ("norm",))
-    return tuple(got) if per_tensor else got[0]
+    code = _norm_code(norm_type)
+    got = _binding().grad_norm(_as_list(grads, "grads"), code, True, bool(per_tensor), False)
+    return got if per_tensor else got[0]
 
 
 def grad_norm_total(grads, norm_type: float = 2.0):
     """What grad_norm takes the norm of, a 0-d float64 tensor: the sum of
     squares, or for inf the largest magnitude. Totals of lists on several
     devices are added (or the largest taken) and given to clip_grad_norm."""
-    return _grad_norm(grads, norm_type, ("total",))[0]
-
-
-def _outputs(grads, out, dev):
-    """The output tensors: new ones, or `out` checked against the inputs."""
-    if out is None:
-        return [torch.empty_like(g) for g in grads]
-    if isinstance(out, torch.Tensor):
-        raise TypeError("out must be a sequence of tensors, not one tensor")
-    out = list(out)
-    if len(out) != len(grads):
-        raise RuntimeError(f"out must hold {len(grads)} tensors, got {len(out)}")
-    for g, o in zip(grads, out):
-        if o is g:
-            pass
-        elif not isinstance(o, torch.Tensor):
-            raise TypeError(f"out must hold tensors, not {type(o).__name__}")
-        elif o.shape != g.shape or o.dtype != g.dtype or o.device != dev:
-            raise RuntimeError(f"out must have the gradients' shape, dtype and device: {tuple(g.shape)} {g.dtype} "
-                               f"{dev}, got {tuple(o.shape)} {o.dtype} {o.device}")
-        if o.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("out must not require grad: clipping is not differentiable")
-        if not o.is_contiguous() and not _one_to_a_place(o):
-            raise RuntimeError("out must hold tensors whose values each have a place of their own")
-    return out
-
-
-def _written(out):
-    # autograd's count of in-place changes, as for torch's own operations
-    kept = [o for o in out if not o.is_inference()]
-    if kept:
-        torch.autograd.graph.increment_version(kept)
+    code = _norm_code(norm_type)
+    return _binding().grad_norm(_as_list(grads, "grads"), code, False, False, True)[0]
 
 
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6, total=None, out=None):
@@ -1135,66 +1033,12 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 
     over all of them together (as grad_norm, or from `total`, a 0-d float64
     tensor on their device as grad_norm_total returns). Returns (the scaled
     gradients, norm): new tensors, or `out` where given; out=grads scales in
-    place. A bound of inf changes nothing; a NaN norm makes every value NaN,
-    an infinite one 0 or NaN."""
+    place. No output may share memory with another tensor of the call. A bound
+    of inf changes nothing; a NaN norm makes every value NaN, an infinite one 0
+    or NaN. The outputs carry no autograd history."""
     code = _norm_code(norm_type)
     max_norm, eps = _bound(max_norm, eps)
-    grads, dev = _grad_list(grads, "grads")
-    if not grads:
-        raise RuntimeError("grads is empty: there is no device to put its norm on")
-    if total is not None:
-        _req(total, "total", (), dev, torch.float64)
-    L = lib()
-    with _on(dev):
-        _device_ok(dev)
-        fresh = out is None
-        out = _outputs(grads, out, dev)
-        src, dst, back = [], [], []
-        for g, o in zip(grads, out):
-            if _without_gaps(g) and (o is g or (o.stride() == g.stride() and not o.is_neg())) and not g.is_neg():
-                src.append(g)
-                dst.append(o)
-            else:
-                flat = _gathered(g)
-                src.append(flat)
-                dst.append(flat)
-                back.append((o, flat))
-        n = len(src)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        nbytes = _grad_workspace_bytes(n)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        ptrs, sizes, types = _arrays(src)
-        outs = array("Q", [t.data_ptr() for t in dst])
-        st = L.ilqr_b200_grad_clip(_at(ptrs), _at(outs), _at(sizes), _at(types), n, code, max_norm, eps, _ptr(total),
-                                   norm.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
-        _check(st, "ilqr_b200_grad_clip")
-        for o, flat in back:
-            o.copy_(flat)
-    if not fresh:
-        _written(out)
-    return out, norm
-
-
-def _segments(g, o, d):
-    """How the slices of g and o along dimension d lie in memory: (segments,
-    their length, strides of g's segments and slices, of o's), in values; None
-    where a slice is not evenly spaced segments of both."""
-    dims = []
-    for k in range(g.dim() - 1, -1, -1):
-        size, gs, os_ = g.shape[k], g.stride(k), o.stride(k)
-        if k == d or size == 1:
-            continue
-        if dims and gs == dims[-1][1] * dims[-1][0] and os_ == dims[-1][2] * dims[-1][0]:
-            dims[-1][0] *= size
-        else:
-            dims.append([size, gs, os_])
-    length = 1
-    if dims and dims[0][1] == 1 and dims[0][2] == 1:
-        length = dims.pop(0)[0]
-    if len(dims) > 1:
-        return None
-    n_seg, gs, os_ = dims[0] if dims else (1, 0, 0)
-    return n_seg, length, gs, g.stride(d), os_, o.stride(d)
+    return _binding().clip_grad_norm(_as_list(grads, "grads"), out, max_norm, code, eps, total)
 
 
 def clip_grad_elements(grads, max_norm: float, batch_dims=0, eps: float = 1e-6, zero_nonfinite: bool = False, out=None):
@@ -1204,47 +1048,11 @@ def clip_grad_elements(grads, max_norm: float, batch_dims=0, eps: float = 1e-6, 
     norms[b] the 2-norm over them, and they are scaled by
     min(1, max_norm / (norms[b] + eps)). The elements of a batch are separate
     solves, so one that diverges leaves the others' gradients as they are. Its
-    own become NaN, or with zero_nonfinite zero. Returns (the scaled gradients,
-    norms [B] float32); out as in clip_grad_norm."""
+    own become NaN (or 0, where its norm is infinite), or with zero_nonfinite
+    zero. Returns (the scaled gradients, norms [B] float32); out as in
+    clip_grad_norm."""
     max_norm, eps = _bound(max_norm, eps)
-    grads, dev = _grad_list(grads, "grads")
-    if not 1 <= len(grads) <= MAX_ELEMENT_TENSORS:
-        raise RuntimeError(f"grads must hold 1 to {MAX_ELEMENT_TENSORS} tensors, got {len(grads)}")
-    dims = [batch_dims] * len(grads) if isinstance(batch_dims, int) else [int(d) for d in batch_dims]
-    if len(dims) != len(grads):
-        raise RuntimeError(f"batch_dims must hold {len(grads)} numbers, got {len(dims)}")
-    for g, d in zip(grads, dims):
-        if not 0 <= d < g.dim():
-            raise RuntimeError(f"batch dimension {d} of a tensor of shape {tuple(g.shape)}")
-    B = grads[0].shape[dims[0]]
-    if any(g.shape[d] != B for g, d in zip(grads, dims)):
-        raise RuntimeError(f"grads must have one batch size, got {[g.shape[d] for g, d in zip(grads, dims)]}")
-    L = lib()
-    with _on(dev):
-        _device_ok(dev)
-        fresh = out is None
-        out = _outputs(grads, out, dev)
-        src, dst, back, layout = [], [], [], array("q")
-        for g, o, d in zip(grads, out, dims):
-            seg = None if g.is_neg() or o.is_neg() else _segments(g, o, d)
-            if seg is None:
-                flat = _gathered(g)
-                src.append(flat)
-                dst.append(flat)
-                back.append((o, flat))
-                seg = _segments(flat, flat, d)
-            else:
-                src.append(g)
-                dst.append(o)
-            layout.extend(seg)
-        norms = torch.empty(B, dtype=torch.float32, device=dev)
-        ptrs, _, types = _arrays(src)
-        outs = array("Q", [t.data_ptr() for t in dst])
-        st = L.ilqr_b200_grad_clip_elements(_at(ptrs), _at(outs), _at(types), _at(layout), len(src), B, max_norm, eps,
-                                            1 if zero_nonfinite else 0, norms.data_ptr(), _stream(dev))
-        _check(st, "ilqr_b200_grad_clip_elements")
-        for o, flat in back:
-            o.copy_(flat)
-    if not fresh:
-        _written(out)
-    return out, norms
+    if not isinstance(batch_dims, int):
+        batch_dims = [int(d) for d in batch_dims]
+    return _binding().clip_grad_elements(_as_list(grads, "grads"), out, batch_dims, max_norm, eps,
+                                         bool(zero_nonfinite))

@@ -118,6 +118,10 @@ def test_binding_refusals_without_gpu():
         nat.grad_norm([x])
     with pytest.raises(RuntimeError, match="empty"):
         nat.grad_norm([])
+    with pytest.raises(RuntimeError, match="empty"):
+        nat.clip_grad_norm(iter([]), 1.0)
+    with pytest.raises(RuntimeError, match="1 to 8"):
+        nat.clip_grad_elements([], 1.0)
     with pytest.raises(ValueError, match="norm_type"):
         nat.grad_norm([x], norm_type=1.0)
     with pytest.raises(ValueError, match="max_norm"):
@@ -132,38 +136,6 @@ def test_binding_refusals_without_gpu():
         nat.clip_grad_elements([x], 1.0)
     with pytest.raises(ValueError, match="max_norm"):
         nat.clip_grad_elements([x], math.nan)
-
-
-def test_how_slices_lie_in_memory():
-    """Batch-major, time-major, permuted and strided gradients as segments."""
-    T, B = 3, 5
-    seg = nat._segments
-    C = torch.empty(B, T, 14, 14)
-    assert seg(C, C, 0) == (1, T * 196, 0, T * 196, 0, T * 196)
-    Ct = torch.empty(T, B, 14, 14)
-    assert seg(Ct, Ct, 1) == (T, 196, B * 196, 196, B * 196, 196)
-    v = Ct.permute(1, 0, 2, 3)
-    assert seg(v, v, 0) == (T, 196, B * 196, 196, B * 196, 196)
-    assert seg(v, C, 0) == (T, 196, B * 196, 196, 196, T * 196)
-    packed = torch.empty(B, 30)
-    assert seg(packed[:, 10:24], packed[:, 10:24], 0) == (1, 14, 0, 30, 0, 30)
-    assert seg(torch.empty(B), torch.empty(B), 0)[:2] == (1, 1)
-    last = torch.empty(7, B)
-    assert seg(last, last, 1) == (7, 1, B, 1, B, 1)
-    wide = torch.empty(B, 6, 8, 10)[:, ::2, ::2, :]
-    assert seg(wide, wide, 0) is None
-    one = torch.empty(1).expand(B, 4)
-    assert seg(one, torch.empty(B, 4), 0) == (4, 1, 0, 0, 1, 4)
-    assert seg(torch.empty(B, 0, 3), torch.empty(B, 0, 3), 0)[0:2].count(0) == 1
-
-
-def test_which_tensors_have_gaps():
-    x = torch.empty(4, 6, 5)
-    assert nat._without_gaps(x) and nat._without_gaps(x.permute(2, 0, 1)) and nat._without_gaps(x[1:3])
-    assert nat._without_gaps(torch.empty(())) and nat._without_gaps(torch.empty(0, 3))
-    assert not nat._without_gaps(x[:, 1:]) and not nat._without_gaps(torch.empty(3).expand(2, 3))
-    assert nat._one_to_a_place(x[:, 1:]) and not nat._one_to_a_place(torch.empty(3).expand(2, 3))
-    assert not nat._one_to_a_place(torch.empty(9).as_strided((4, 3), (2, 1)))
 
 
 # ---- the paths' host logic ---------------------------------------------------
