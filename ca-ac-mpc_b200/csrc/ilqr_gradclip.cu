@@ -439,34 +439,63 @@ __device__ __forceinline__ Vec<VB> pack_vec(const float* x) {
   return v;
 }
 
-template <int DT, int VB>
-__device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, uint32_t lane, uint32_t step) {
+// Vector i of a slice lies in segment i / seg_vecs: by a multiplication with
+// the reciprocal rounded up to 2^(31 + shift), exact for i < 2^31.
+__device__ __forceinline__ int64_t vec_at(const RowTensor& r, uint32_t i, uint32_t vb, int64_t seg_stride) {
+  if (r.n_seg == 1) return (int64_t)i * vb;
+  const uint32_t s = r.seg_vecs == 1 ? i : __umulhi(i, r.magic) >> r.shift;
+  return s * seg_stride + (int64_t)(i - s * r.seg_vecs) * vb;
+}
+
+template <int VB>
+__device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
+  if constexpr (VB == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  } else if constexpr (VB == 2) {
+    const uint16_t w = *reinterpret_cast<const uint16_t*>(from);
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(w) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(VB) : "memory");
+  }
+}
+
+// The three steps of a slice. Each thread copies, adds and scales the same
+// vectors: no thread reads what another copied, so the copies need no barrier.
+template <int VB>
+__device__ __forceinline__ void row_copy(const RowTensor& r, int64_t b, uint32_t to, uint32_t lane, uint32_t step) {
+  const char* p = r.in + b * r.in_row;
+  const uint32_t n = r.n_seg * r.seg_vecs;
+  for (uint32_t i = lane; i < n; i += step) copy_async<VB>(to + i * VB, p + vec_at(r, i, VB, r.in_seg));
+}
+
+template <int DT, int VB, bool STAGED>
+__device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, const char* staged, uint32_t lane,
+                                        uint32_t step) {
   constexpr int NV = VB / Type<DT>::SIZE;
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
   for (uint32_t i = lane; i < n; i += step) {
-    const uint32_t s = r.n_seg == 1 ? 0 : i / r.seg_vecs;
+    const char* at = STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg);
     float x[NV < 2 ? 2 : NV];
-    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(p + s * r.in_seg + (int64_t)(i - s * r.seg_vecs) * VB), x);
+    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(at), x);
     add<DT, NV>(a, x);
   }
 }
 
-template <int DT, int VB>
-__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const Coef& c, bool zero, uint32_t lane,
-                                          uint32_t step) {
+template <int DT, int VB, bool STAGED>
+__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const char* staged, const Coef& c, bool zero,
+                                          uint32_t lane, uint32_t step) {
   constexpr int NV = VB / Type<DT>::SIZE;
   const char* p = r.in + b * r.in_row;
   char* q = r.out + b * r.out_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
   for (uint32_t i = lane; i < n; i += step) {
-    const uint32_t s = r.n_seg == 1 ? 0 : i / r.seg_vecs;
-    const int64_t off = (int64_t)(i - s * r.seg_vecs) * VB;
+    const char* at = STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg);
     float x[NV < 2 ? 2 : NV];
-    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(p + s * r.in_seg + off), x);
+    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(at), x);
 #pragma unroll
     for (int j = 0; j < NV; ++j) x[j] = zero ? 0.0f : scaled(x[j], c);
-    *reinterpret_cast<Vec<VB>*>(q + s * r.out_seg + off) = pack_vec<DT, VB>(x);
+    *reinterpret_cast<Vec<VB>*>(q + vec_at(r, i, VB, r.out_seg)) = pack_vec<DT, VB>(x);
   }
 }
 
@@ -485,29 +514,44 @@ __device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const C
     default: CALL(ILQR_DTYPE_BF16, 2); break;                                       \
   }
 
-// A warp (ONE_WARP) or a block for each element.
-template <bool ONE_WARP>
-__global__ void __launch_bounds__(NT) grad_rows_kernel(const __grid_constant__ RowTable tab) {
+// G threads (a warp or the block) for each element. STAGED: its slices are
+// copied to shared memory, read from there twice and written once, so global
+// memory is read once; without, both passes read global memory.
+template <int G, int THREADS, bool STAGED>
+__global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constant__ RowTable tab) {
+  extern __shared__ __align__(16) char staged[];
   __shared__ double sh[32];
-  const int64_t b = ONE_WARP ? (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  if (b >= tab.B) return;
-  const uint32_t lane = ONE_WARP ? threadIdx.x & 31 : threadIdx.x;
-  constexpr uint32_t step = ONE_WARP ? 32 : NT;
+  constexpr int PER = THREADS / G;
+  const int64_t b = PER == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * PER + threadIdx.x / G;
+  if (b >= tab.B) return;  // of a whole warp, or not at all
+  const uint32_t lane = threadIdx.x % G;
+  const char* mine = staged + (PER == 1 ? 0 : (threadIdx.x / G) * tab.staged_bytes);
+  if (STAGED) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine);
+    for (int k = 0; k < tab.n; ++k) {
+      const RowTensor& r = tab.t[k];
+      if (r.vec_bytes == 16) row_copy<16>(r, b, to + r.staged, lane, G);
+      else if (r.vec_bytes == 8) row_copy<8>(r, b, to + r.staged, lane, G);
+      else if (r.vec_bytes == 4) row_copy<4>(r, b, to + r.staged, lane, G);
+      else row_copy<2>(r, b, to + r.staged, lane, G);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
   Acc<false> a;
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tab.t[k];
-#define CALL(DT, VB) row_sum<DT, VB>(a, r, b, lane, step)
+#define CALL(DT, VB) row_sum<DT, VB, STAGED>(a, r, b, mine + r.staged, lane, G)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
-  const double nrm = sqrt(ONE_WARP ? warp_join<false>(a.s) : block_join<false>(a.s, sh));
+  const double nrm = sqrt(G == 32 ? warp_join<false>(a.s) : block_join<false>(a.s, sh));
   if (lane == 0 && tab.norms != nullptr) tab.norms[b] = (float)nrm;
   const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
   const bool zero = tab.zero_nonfinite && !isfinite(nrm);
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tab.t[k];
     if (c.d == 1.0 && !zero && r.in == r.out) continue;
-#define CALL(DT, VB) row_scale<DT, VB>(r, b, c, zero, lane, step)
+#define CALL(DT, VB) row_scale<DT, VB, STAGED>(r, b, mine + r.staged, c, zero, lane, G)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
@@ -570,10 +614,32 @@ INSTANTIATE(GRAD_CAP_SHORT)
 INSTANTIATE(GRAD_CAP_LONG)
 #undef INSTANTIATE
 
-cudaError_t launch_grad_rows(const RowTable& tab, int64_t row_bytes, cudaStream_t stream) {
-  if (row_bytes <= 4096)
-    return launch(grad_rows_kernel<true>, (unsigned)((tab.B + NT / 32 - 1) / (NT / 32)), false, stream, tab);
-  return launch(grad_rows_kernel<false>, (unsigned)tab.B, false, stream, tab);
+namespace {
+
+template <int G, int THREADS, bool STAGED>
+cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream) {
+  constexpr int PER = THREADS / G;
+  const size_t smem = STAGED ? (size_t)tab.staged_bytes * PER : 0;
+  const auto kernel = grad_rows_kernel<G, THREADS, STAGED>;
+  if (STAGED) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((tab.B + PER - 1) / PER));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, tab);
+}
+
+}  // namespace
+
+cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
+  if (tab.staged_bytes <= 4096) return launch_rows<32, 128, true>(tab, stream);
+  if (tab.staged_bytes <= 20480) return launch_rows<128, 128, true>(tab, stream);
+  if (tab.staged_bytes <= 220000) return launch_rows<256, 256, true>(tab, stream);
+  return launch_rows<256, 256, false>(tab, stream);
 }
 
 }  // namespace ilqr

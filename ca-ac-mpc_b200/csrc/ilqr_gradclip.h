@@ -59,6 +59,9 @@ struct RowTensor {
   int64_t in_row, in_seg, out_row, out_seg;
   uint32_t n_seg, seg_vecs;
   uint32_t vec_bytes, dtype;
+  uint32_t magic, shift;  // i / seg_vecs = i magic >> (32 + shift)
+  uint32_t staged;        // where the slice is staged, from the element's place
+  uint32_t pad;
 };
 
 constexpr int ROW_MAX_TENSORS = 8;
@@ -70,6 +73,8 @@ struct RowTable {
   int64_t B;
   double max_norm, eps;
   float* norms;
+  uint32_t staged_bytes;  // of an element, every slice from a multiple of 16
+  uint32_t pad;
 };
 
 template <int CAP>
@@ -84,7 +89,7 @@ cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* 
 template <int CAP>
 cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
                               int64_t n_slots, float* norm, bool dependent, cudaStream_t stream);
-cudaError_t launch_grad_rows(const RowTable& tab, int64_t row_bytes, cudaStream_t stream);
+cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream);
 
 }  // namespace ilqr
 

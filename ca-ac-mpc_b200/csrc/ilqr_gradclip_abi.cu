@@ -266,6 +266,16 @@ bool disjoint(const Rows& a, const Rows& b) {
   return at >= x.len && at + y.len <= x.row;
 }
 
+// i / d = i magic >> (32 + shift) for 0 <= i < 2^31 and d >= 2: with
+// 2^shift < d <= 2^(shift + 1) and magic = ceil(2^(32 + shift) / d) < 2^32 the
+// error magic d - 2^(32 + shift) is below d, and i times it below 2^(32 + shift).
+void reciprocal(uint32_t d, uint32_t* magic, uint32_t* shift) {
+  *magic = *shift = 0;
+  if (d < 2) return;
+  while (((uint64_t)2 << *shift) < d) ++*shift;
+  *magic = (uint32_t)((((uint64_t)1 << (32 + *shift)) + d - 1) / d);
+}
+
 bool same(const Rows& a, const Rows& b) {
   return a.base == b.base && (a.B == 1 || a.row == b.row) && (a.n_seg == 1 || a.seg == b.seg);
 }
@@ -313,10 +323,16 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
     if (n_seg > 1) all |= (uintptr_t)ins[k].seg | (uintptr_t)outs[k].seg;
     if (B > 1) all |= (uintptr_t)ins[k].row | (uintptr_t)outs[k].row;
     const uint32_t vec = (uint32_t)(all & (~all + 1));
-    tab.t[k] = ilqr::RowTensor{static_cast<const char*>(grads[i]), static_cast<char*>(out[i]), ins[k].row, ins[k].seg,
-                               outs[k].row, outs[k].seg, (uint32_t)n_seg, (uint32_t)(len * sz / vec), vec,
-                               (uint32_t)dtypes[i]};
-    row_bytes += n_seg * len * sz;
+    ilqr::RowTensor& r = tab.t[k];
+    r.in = static_cast<const char*>(grads[i]);
+    r.out = static_cast<char*>(out[i]);
+    r.in_row = ins[k].row, r.in_seg = ins[k].seg;
+    r.out_row = outs[k].row, r.out_seg = outs[k].seg;
+    r.n_seg = (uint32_t)n_seg, r.seg_vecs = (uint32_t)(len * sz / vec);
+    r.vec_bytes = vec, r.dtype = (uint32_t)dtypes[i];
+    reciprocal(r.seg_vecs, &r.magic, &r.shift);
+    r.staged = (uint32_t)std::min<int64_t>(row_bytes, UINT32_MAX);
+    row_bytes += (n_seg * len * sz + 15) / 16 * 16;
   }
   for (int a = 0; a < tab.n; ++a)
     for (int b = 0; b < tab.n; ++b) {
@@ -329,7 +345,8 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
   tab.eps = eps;
   tab.zero_nonfinite = zero_nonfinite != 0 ? 1 : 0;
   tab.norms = norms;
-  return status_of(ilqr::launch_grad_rows(tab, row_bytes, stream));
+  tab.staged_bytes = (uint32_t)std::min<int64_t>(row_bytes, UINT32_MAX);
+  return status_of(ilqr::launch_grad_rows(tab, stream));
 }
 
 }  // extern "C"
