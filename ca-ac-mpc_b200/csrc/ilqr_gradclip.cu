@@ -4,13 +4,16 @@
 // out = c g. Per batch element: the same over each element's slices of up to
 // eight tensors.
 //
-// Sums: eight values are squared and added in 32 bits, and those sums in 64
-// bits. Eight roundings of relative size 2^-24 at most move a sum of squares by
-// 2^-21, its root by 2^-22, whatever the length. Squares that leave the range
-// of a float (|g| above 2^63, or so small that the group's sum is under 2^-100)
-// are formed again in 64 bits, so a norm is right wherever it is a float
-// itself. The order of every sum is fixed by sizes and grid: no atomics, the
-// same bits each time.
+// Sums: up to 32 values are squared and added in 32 bits, in four or eight
+// chains that are joined in pairs, and those sums in 64 bits. No value passes
+// through more than eight roundings of relative size 2^-24 on the way: they move
+// a sum of squares by 2^-21 at most, its root by 2^-22, whatever the length. (A
+// conversion and an addition in 64 bits for every four values instead cost as
+// much as everything else: the per-element kernel was bound by instructions.)
+// Squares that leave the range of a float (|g| above 2^63, or so small that the
+// group's sum is under 2^-100) are formed again in 64 bits, so a norm is right
+// wherever it is a float itself. The order of every sum is fixed by sizes and
+// grid: no atomics, the same bits each time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -93,14 +96,32 @@ template <> struct Acc<true> {
   uint32_t m = 0u;
 };
 
+// whether a value is not zero
+template <int N>
+__device__ __forceinline__ bool any_of(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m |= __float_as_uint(x[i]) << 1;
+  return m != 0;
+}
+
+// N values (a power of two, 32 at most)
 template <int DT, int N>
 __device__ __forceinline__ void add(Acc<false>& a, const float* x) {
-  float s = 0.0f;
+  constexpr int NC = N >= 32 ? 8 : N >= 4 ? 4 : N;
+  float c[NC];
 #pragma unroll
-  for (int i = 0; i < N; ++i) s = __fmaf_rn(x[i], x[i], s);
+  for (int i = 0; i < NC; ++i) c[i] = __fmul_rn(x[i], x[i]);
+#pragma unroll
+  for (int i = NC; i < N; ++i) c[i % NC] = __fmaf_rn(x[i], x[i], c[i % NC]);
+#pragma unroll
+  for (int o = NC / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) c[i] = __fadd_rn(c[i], c[i + o]);
+  const float s = c[0];
   if (!Type<DT>::WIDE || (s >= 0x1p-100f && s < __int_as_float(0x7f800000))) {
     a.s += (double)s;
-  } else {
+  } else if (s != 0.0f || any_of<N>(x)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) a.s = __fma_rn((double)x[i], (double)x[i], a.s);
   }
@@ -141,10 +162,12 @@ __device__ __forceinline__ double block_join(double v, double* sh) {
 
 __device__ __forceinline__ double norm_of(double total, bool max_type) { return max_type ? total : sqrt(total); }
 
+// WIDE: the coefficient is so small that as a float it has lost bits; the
+// product is formed in 64 bits.
 struct Coef {
   float f;
   double d;
-  bool wide;  // f is so small that it has lost bits: the product is formed in 64 bits
+  bool wide;
 };
 
 __device__ __forceinline__ Coef coef_of(double norm, double max_norm, double eps) {
@@ -156,30 +179,80 @@ __device__ __forceinline__ Coef coef_of(double norm, double max_norm, double eps
   return c;
 }
 
+template <bool WIDE>
 __device__ __forceinline__ float scaled(float x, const Coef& c) {
-  return c.wide ? (float)((double)x * c.d) : x * c.f;
+  if constexpr (WIDE) return (float)((double)x * c.d);
+  return x * c.f;
+}
+
+// ---- vectors ---------------------------------------------------------------
+
+template <int VB> struct Vec;
+template <> struct Vec<16> { uint4 w; };
+template <> struct Vec<8> { uint2 w; };
+template <> struct Vec<4> { uint32_t w; };
+template <> struct Vec<2> { uint16_t w; };
+
+template <int VB>
+__device__ __forceinline__ Vec<VB> load_vec(const char* p) {
+  return *reinterpret_cast<const Vec<VB>*>(p);
+}
+
+template <int DT, int VB>
+__device__ __forceinline__ void unpack_vec(const Vec<VB>& v, float* x) {
+  if constexpr (VB == 2) {
+    float two[2];
+    unpack<DT>((uint32_t)v.w, two);
+    x[0] = two[0];
+  } else {
+    constexpr int K = 4 / Type<DT>::SIZE;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < VB / 4; ++k) unpack<DT>(w[k], x + k * K);
+  }
+}
+
+template <int DT, int VB>
+__device__ __forceinline__ Vec<VB> pack_vec(const float* x) {
+  Vec<VB> v;
+  if constexpr (VB == 2) {
+    const float two[2] = {x[0], 0.0f};
+    v.w = (uint16_t)pack<DT>(two);
+  } else {
+    constexpr int K = 4 / Type<DT>::SIZE;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < VB / 4; ++k) w[k] = pack<DT>(x + k * K);
+  }
+  return v;
+}
+
+// U vectors into a sum
+template <int DT, int VB, int U, bool MAX>
+__device__ __forceinline__ void add_vecs(Acc<MAX>& a, const Vec<VB>* v) {
+  constexpr int NV = VB / Type<DT>::SIZE;
+  float x[U * NV];
+#pragma unroll
+  for (int u = 0; u < U; ++u) unpack_vec<DT, VB>(v[u], x + u * NV);
+  add<DT, U * NV>(a, x);
+}
+
+template <int DT, int VB, bool WIDE>
+__device__ __forceinline__ Vec<VB> scale_vec(const Vec<VB>& v, const Coef& c) {
+  constexpr int NV = VB / Type<DT>::SIZE;
+  float x[NV];
+  unpack_vec<DT, VB>(v, x);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) x[j] = scaled<WIDE>(x[j], c);
+  return pack_vec<DT, VB>(x);
 }
 
 // ---- a range of a dense tensor ---------------------------------------------
-
-__device__ __forceinline__ uint4 load16(const char* p) { return *reinterpret_cast<const uint4*>(p); }
 
 template <int DT>
 __device__ __forceinline__ int head_of(const char* p, int64_t n) {
   const int h = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / Type<DT>::SIZE;
   return n < h ? (int)n : h;
-}
-
-template <int DT, bool MAX>
-__device__ __forceinline__ void add_vec(Acc<MAX>& a, const uint4& v) {
-  float x[8];
-  if constexpr (DT == ILQR_DTYPE_F32) {
-    unpack<DT>(v.x, x), unpack<DT>(v.y, x + 1), unpack<DT>(v.z, x + 2), unpack<DT>(v.w, x + 3);
-    add<DT, 4>(a, x);
-  } else {
-    unpack<DT>(v.x, x), unpack<DT>(v.y, x + 2), unpack<DT>(v.z, x + 4), unpack<DT>(v.w, x + 6);
-    add<DT, 8>(a, x);
-  }
 }
 
 template <int DT, bool MAX>
@@ -195,13 +268,13 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   n -= h;
   const int64_t nv = n / VE;
   for (int64_t i = tid; i < nv; i += UN * NT) {
-    uint4 v[UN];
+    Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
-      if (i + u * NT < nv) v[u] = load16(p + (i + u * NT) * 16);
-#pragma unroll
-    for (int u = 0; u < UN; ++u)
-      if (i + u * NT < nv) add_vec<DT, MAX>(a, v[u]);
+    for (int u = 0; u < UN; ++u) {
+      v[u].w = make_uint4(0, 0, 0, 0);
+      if (i + u * NT < nv) v[u] = load_vec<16>(p + (i + u * NT) * 16);
+    }
+    add_vecs<DT, 16, UN, MAX>(a, v);
   }
   const int tail = (int)(n - nv * VE);
   if (tid < tail) {
@@ -210,62 +283,51 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   }
 }
 
+// out = c in, value by value: `in` and `out` that lie differently in their
+// 16-byte words, and coefficients below the floats' range.
 template <int DT>
-__device__ __forceinline__ uint4 scale_vec(const uint4& v, const Coef& c) {
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __noinline__ void range_scale_apart(const char* p, char* q, int64_t n, const Coef& c) {
+  constexpr int SZ = Type<DT>::SIZE;
+#pragma unroll 1
+  for (int64_t i = threadIdx.x; i < n; i += 4 * NT) {
+    float x[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float x[2];
-    unpack<DT>(w[k], x);
+    for (int u = 0; u < 4; ++u)
+      if (i + u * NT < n) x[u] = load_one<DT>(p + (i + u * NT) * SZ);
 #pragma unroll
-    for (int j = 0; j < 4 / Type<DT>::SIZE; ++j) x[j] = scaled(x[j], c);
-    w[k] = pack<DT>(x);
+    for (int u = 0; u < 4; ++u)
+      if (i + u * NT < n) store_one<DT>(q + (i + u * NT) * SZ, c.wide ? scaled<true>(x[u], c) : scaled<false>(x[u], c));
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // out = c in; `in` may be `out`
 template <int DT>
 __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
+  if (c.wide || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u)) {
+    range_scale_apart<DT>(p, q, n, c);
+    return;
+  }
   const int tid = threadIdx.x;
   const int h = head_of<DT>(p, n);
-  if (tid < h) store_one<DT>(q + tid * SZ, scaled(load_one<DT>(p + tid * SZ), c));
+  if (tid < h) store_one<DT>(q + tid * SZ, scaled<false>(load_one<DT>(p + tid * SZ), c));
   p += h * SZ;
   q += h * SZ;
   n -= h;
-  const bool together = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
   const int64_t nv = n / VE;
   for (int64_t i = tid; i < nv; i += UN * NT) {
-    uint4 v[UN];
+    Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (i + u * NT < nv) v[u] = load16(p + (i + u * NT) * 16);
+      if (i + u * NT < nv) v[u] = load_vec<16>(p + (i + u * NT) * 16);
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      if (i + u * NT >= nv) continue;
-      const uint4 y = scale_vec<DT>(v[u], c);
-      char* to = q + (i + u * NT) * 16;
-      if (together) {
-        *reinterpret_cast<uint4*>(to) = y;
-      } else {
-        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (SZ == 4) {
-            reinterpret_cast<uint32_t*>(to)[k] = w[k];
-          } else {
-            reinterpret_cast<uint16_t*>(to)[2 * k] = (uint16_t)w[k];
-            reinterpret_cast<uint16_t*>(to)[2 * k + 1] = (uint16_t)(w[k] >> 16);
-          }
-        }
-      }
-    }
+    for (int u = 0; u < UN; ++u)
+      if (i + u * NT < nv) *reinterpret_cast<Vec<16>*>(q + (i + u * NT) * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
   const int tail = (int)(n - nv * VE);
   if (tid < tail) {
     const int64_t at = (nv * VE + tid) * SZ;
-    store_one<DT>(q + at, scaled(load_one<DT>(p + at), c));
+    store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
   }
 }
 
@@ -308,6 +370,15 @@ __device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const voi
   if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX>(a, p + at * 4, n);
   else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX>(a, p + at * 2, n);
   else range_sum<ILQR_DTYPE_F16, MAX>(a, p + at * 2, n);
+}
+
+__device__ __forceinline__ void entry_scale(uint32_t dtype, const void* in, void* out, int64_t at, int64_t n,
+                                            const Coef& c) {
+  const char* p = static_cast<const char*>(in);
+  char* q = static_cast<char*>(out);
+  if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p + at * 4, q + at * 4, n, c);
+  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p + at * 2, q + at * 2, n, c);
+  else range_scale<ILQR_DTYPE_F16>(p + at * 2, q + at * 2, n, c);
 }
 
 // Partial sums. Each block takes a contiguous run of chunks; with PER one sum
@@ -377,7 +448,7 @@ __global__ void __launch_bounds__(NT) grad_join_kernel(const __grid_constant__ G
 // out = c in over the list; every block joins the partial sums for itself, in
 // the same order. In place a coefficient of 1 leaves the values where they are.
 template <int CAP>
-__global__ void __launch_bounds__(NT) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
+__global__ void __launch_bounds__(NT, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
                                                         const double* slots, int64_t n_slots, float* norm) {
   __shared__ double sh[32];
   uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
@@ -394,50 +465,13 @@ __global__ void __launch_bounds__(NT) grad_scale_kernel(const __grid_constant__ 
     if (!(c.d == 1.0 && e.in == e.out)) {
       int64_t at, n;
       span(tab, t, k, end, &at, &n);
-      const char* p = static_cast<const char*>(e.in);
-      char* q = static_cast<char*>(e.out);
-      if (e.dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p + at * 4, q + at * 4, n, c);
-      else if (e.dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p + at * 2, q + at * 2, n, c);
-      else range_scale<ILQR_DTYPE_F16>(p + at * 2, q + at * 2, n, c);
+      entry_scale(e.dtype, e.in, e.out, at, n, c);
     }
     k = end;
   }
 }
 
 // ---- batch elements ---------------------------------------------------------
-
-template <int VB> struct Vec;
-template <> struct Vec<16> { uint4 w; };
-template <> struct Vec<8> { uint2 w; };
-template <> struct Vec<4> { uint32_t w; };
-template <> struct Vec<2> { uint16_t w; };
-
-template <int DT, int VB>
-__device__ __forceinline__ void unpack_vec(const Vec<VB>& v, float* x) {
-  if constexpr (VB == 2) {
-    unpack<DT>((uint32_t)v.w, x);
-  } else {
-    constexpr int K = 4 / Type<DT>::SIZE;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-    for (int k = 0; k < VB / 4; ++k) unpack<DT>(w[k], x + k * K);
-  }
-}
-
-template <int DT, int VB>
-__device__ __forceinline__ Vec<VB> pack_vec(const float* x) {
-  Vec<VB> v;
-  if constexpr (VB == 2) {
-    const float two[2] = {x[0], 0.0f};
-    v.w = (uint16_t)pack<DT>(two);
-  } else {
-    constexpr int K = 4 / Type<DT>::SIZE;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-    for (int k = 0; k < VB / 4; ++k) w[k] = pack<DT>(x + k * K);
-  }
-  return v;
-}
 
 // Vector i of a slice lies in segment i / seg_vecs: by a multiplication with
 // the reciprocal rounded up to 2^(31 + shift), exact for i < 2^31.
@@ -465,37 +499,61 @@ template <int VB>
 __device__ __forceinline__ void row_copy(const RowTensor& r, int64_t b, uint32_t to, uint32_t lane, uint32_t step) {
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
+#pragma unroll 4
   for (uint32_t i = lane; i < n; i += step) copy_async<VB>(to + i * VB, p + vec_at(r, i, VB, r.in_seg));
 }
 
 template <int DT, int VB, bool STAGED>
 __device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, const char* staged, uint32_t lane,
                                         uint32_t step) {
-  constexpr int NV = VB / Type<DT>::SIZE;
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
-  for (uint32_t i = lane; i < n; i += step) {
-    const char* at = STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg);
-    float x[NV < 2 ? 2 : NV];
-    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(at), x);
-    add<DT, NV>(a, x);
+  for (uint32_t i = lane; i < n; i += UN * step) {
+    Vec<VB> v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const uint32_t k = i + u * step;
+      v[u] = Vec<VB>{};
+      if (k < n) v[u] = load_vec<VB>(STAGED ? staged + k * VB : p + vec_at(r, k, VB, r.in_seg));
+    }
+    add_vecs<DT, VB, UN, false>(a, v);
   }
 }
 
 template <int DT, int VB, bool STAGED>
-__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const char* staged, const Coef& c, bool zero,
+__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const char* staged, const Coef& c,
                                           uint32_t lane, uint32_t step) {
-  constexpr int NV = VB / Type<DT>::SIZE;
   const char* p = r.in + b * r.in_row;
   char* q = r.out + b * r.out_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
+#pragma unroll 4
   for (uint32_t i = lane; i < n; i += step) {
-    const char* at = STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg);
-    float x[NV < 2 ? 2 : NV];
-    unpack_vec<DT, VB>(*reinterpret_cast<const Vec<VB>*>(at), x);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) x[j] = zero ? 0.0f : scaled(x[j], c);
-    *reinterpret_cast<Vec<VB>*>(q + vec_at(r, i, VB, r.out_seg)) = pack_vec<DT, VB>(x);
+    const Vec<VB> v = load_vec<VB>(STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg));
+    *reinterpret_cast<Vec<VB>*>(q + vec_at(r, i, VB, r.out_seg)) = scale_vec<DT, VB, false>(v, c);
+  }
+}
+
+// Value by value: zeros in the place of a slice, or coefficients below the
+// floats' range.
+__device__ __noinline__ void row_apart(const RowTensor& r, int64_t b, const Coef& c, bool zero, uint32_t lane,
+                                       uint32_t step) {
+  const uint32_t sz = r.dtype == ILQR_DTYPE_F32 ? 4 : 2, per = r.vec_bytes / sz;
+  const char* p = r.in + b * r.in_row;
+  char* q = r.out + b * r.out_row;
+  const uint32_t n = r.n_seg * r.seg_vecs;
+#pragma unroll 1
+  for (uint32_t i = lane; i < n; i += step) {
+    const char* from = p + vec_at(r, i, r.vec_bytes, r.in_seg);
+    char* to = q + vec_at(r, i, r.vec_bytes, r.out_seg);
+#pragma unroll 1
+    for (uint32_t k = 0; k < per; ++k, from += sz, to += sz) {
+      if (r.dtype == ILQR_DTYPE_F32)
+        store_one<ILQR_DTYPE_F32>(to, zero ? 0.0f : scaled<true>(load_one<ILQR_DTYPE_F32>(from), c));
+      else if (r.dtype == ILQR_DTYPE_BF16)
+        store_one<ILQR_DTYPE_BF16>(to, zero ? 0.0f : scaled<true>(load_one<ILQR_DTYPE_BF16>(from), c));
+      else
+        store_one<ILQR_DTYPE_F16>(to, zero ? 0.0f : scaled<true>(load_one<ILQR_DTYPE_F16>(from), c));
+    }
   }
 }
 
@@ -551,7 +609,11 @@ __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constan
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tab.t[k];
     if (c.d == 1.0 && !zero && r.in == r.out) continue;
-#define CALL(DT, VB) row_scale<DT, VB, STAGED>(r, b, mine + r.staged, c, zero, lane, G)
+    if (zero || c.wide) {
+      row_apart(r, b, c, zero, lane, G);
+      continue;
+    }
+#define CALL(DT, VB) row_scale<DT, VB, STAGED>(r, b, mine + r.staged, c, lane, G)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
