@@ -260,43 +260,27 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
   const int tid = threadIdx.x;
   const int h = head_of<DT>(p, n);
-  if (tid < h) {
-    const float x = load_one<DT>(p + tid * SZ);
+  const int tail = (int)((n - h) % VE);
+  if (tid < h + tail) {
+    const float x = load_one<DT>(p + (tid < h ? tid : n - tail + (tid - h)) * SZ);
     add<DT, 1>(a, &x);
   }
-  p += h * SZ;
-  n -= h;
-  const int64_t nv = n / VE;
-  for (int64_t i = tid; i < nv; i += UN * NT) {
+  p += h * SZ + tid * 16;
+  int64_t left = (n - h) / VE - tid;  // vectors from this thread's first on
+  for (; left > (UN - 1) * NT; left -= UN * NT, p += UN * NT * 16) {
+    Vec<16> v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * NT * 16);
+    add_vecs<DT, 16, UN, MAX>(a, v);
+  }
+  if (left > 0) {
     Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       v[u].w = make_uint4(0, 0, 0, 0);
-      if (i + u * NT < nv) v[u] = load_vec<16>(p + (i + u * NT) * 16);
+      if (left > u * NT) v[u] = load_vec<16>(p + u * NT * 16);
     }
     add_vecs<DT, 16, UN, MAX>(a, v);
-  }
-  const int tail = (int)(n - nv * VE);
-  if (tid < tail) {
-    const float x = load_one<DT>(p + (nv * VE + tid) * SZ);
-    add<DT, 1>(a, &x);
-  }
-}
-
-// out = c in, value by value: `in` and `out` that lie differently in their
-// 16-byte words, and coefficients below the floats' range.
-template <int DT>
-__device__ __noinline__ void range_scale_apart(const char* p, char* q, int64_t n, const Coef& c) {
-  constexpr int SZ = Type<DT>::SIZE;
-#pragma unroll 1
-  for (int64_t i = threadIdx.x; i < n; i += 4 * NT) {
-    float x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + u * NT < n) x[u] = load_one<DT>(p + (i + u * NT) * SZ);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + u * NT < n) store_one<DT>(q + (i + u * NT) * SZ, c.wide ? scaled<true>(x[u], c) : scaled<false>(x[u], c));
   }
 }
 
@@ -304,30 +288,35 @@ __device__ __noinline__ void range_scale_apart(const char* p, char* q, int64_t n
 template <int DT>
 __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
-  if (c.wide || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u)) {
-    range_scale_apart<DT>(p, q, n, c);
-    return;
-  }
   const int tid = threadIdx.x;
   const int h = head_of<DT>(p, n);
-  if (tid < h) store_one<DT>(q + tid * SZ, scaled<false>(load_one<DT>(p + tid * SZ), c));
-  p += h * SZ;
-  q += h * SZ;
-  n -= h;
-  const int64_t nv = n / VE;
-  for (int64_t i = tid; i < nv; i += UN * NT) {
+  const int tail = (int)((n - h) % VE);
+  if (tid < h + tail) {
+    const int64_t at = (tid < h ? tid : n - tail + (tid - h)) * SZ;
+    store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
+  }
+  // from the end: what the sums read last is still in L2
+  const int64_t nv = (n - h) / VE, full = nv / (UN * NT) * (UN * NT);
+  int64_t left = nv - full - tid;
+  p += h * SZ + (full + tid) * 16;
+  q += h * SZ + (full + tid) * 16;
+  if (left > 0) {
     Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (i + u * NT < nv) v[u] = load_vec<16>(p + (i + u * NT) * 16);
+      if (left > u * NT) v[u] = load_vec<16>(p + u * NT * 16);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (i + u * NT < nv) *reinterpret_cast<Vec<16>*>(q + (i + u * NT) * 16) = scale_vec<DT, 16, false>(v[u], c);
+      if (left > u * NT) *reinterpret_cast<Vec<16>*>(q + u * NT * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
-  const int tail = (int)(n - nv * VE);
-  if (tid < tail) {
-    const int64_t at = (nv * VE + tid) * SZ;
-    store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
+  for (left = full; left > 0; left -= UN * NT) {
+    p -= UN * NT * 16;
+    q -= UN * NT * 16;
+    Vec<16> v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * NT * 16);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * NT * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
 }
 
@@ -372,13 +361,34 @@ __device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const voi
   else range_sum<ILQR_DTYPE_F16, MAX>(a, p + at * 2, n);
 }
 
+// Value by value: for coefficients below the floats' range, and for `in` and
+// `out` that lie differently in their 16-byte words.
+__device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p, char* q, int64_t n, const Coef& c) {
+  const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
+#pragma unroll 1
+  for (int64_t i = threadIdx.x; i < n; i += NT) {
+    const char* from = p + i * sz;
+    float x = dtype == ILQR_DTYPE_F32    ? load_one<ILQR_DTYPE_F32>(from)
+              : dtype == ILQR_DTYPE_BF16 ? load_one<ILQR_DTYPE_BF16>(from)
+                                         : load_one<ILQR_DTYPE_F16>(from);
+    x = c.wide ? scaled<true>(x, c) : scaled<false>(x, c);
+    char* to = q + i * sz;
+    if (dtype == ILQR_DTYPE_F32) store_one<ILQR_DTYPE_F32>(to, x);
+    else if (dtype == ILQR_DTYPE_BF16) store_one<ILQR_DTYPE_BF16>(to, x);
+    else store_one<ILQR_DTYPE_F16>(to, x);
+  }
+}
+
 __device__ __forceinline__ void entry_scale(uint32_t dtype, const void* in, void* out, int64_t at, int64_t n,
                                             const Coef& c) {
-  const char* p = static_cast<const char*>(in);
-  char* q = static_cast<char*>(out);
-  if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p + at * 4, q + at * 4, n, c);
-  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p + at * 2, q + at * 2, n, c);
-  else range_scale<ILQR_DTYPE_F16>(p + at * 2, q + at * 2, n, c);
+  const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
+  const char* p = static_cast<const char*>(in) + at * sz;
+  char* q = static_cast<char*>(out) + at * sz;
+  if (c.wide || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u))
+    entry_scale_apart(dtype, p, q, n, c);
+  else if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p, q, n, c);
+  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p, q, n, c);
+  else range_scale<ILQR_DTYPE_F16>(p, q, n, c);
 }
 
 // Partial sums. Each block takes a contiguous run of chunks; with PER one sum
@@ -451,23 +461,23 @@ template <int CAP>
 __global__ void __launch_bounds__(NT, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
                                                         const double* slots, int64_t n_slots, float* norm) {
   __shared__ double sh[32];
-  uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
-  const uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
-  int t = find(tab, k);
+  const uint32_t k0 = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
+  uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
+  int t = find(tab, k1 - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const double total = s.max_type ? join_slots<true>(slots, n_slots, sh) : join_slots<false>(slots, n_slots, sh);
   const double nrm = norm_of(total, s.max_type);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
   const Coef c = coef_of(nrm, s.max_norm, s.eps);
-  for (; k < k1; ++t) {
-    const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
+  for (; k1 > k0; --t) {
     const GradEntry& e = tab.e[t];
+    const uint32_t begin = max(k0, e.chunk0);
     if (!(c.d == 1.0 && e.in == e.out)) {
       int64_t at, n;
-      span(tab, t, k, end, &at, &n);
+      span(tab, t, begin, k1, &at, &n);
       entry_scale(e.dtype, e.in, e.out, at, n, c);
     }
-    k = end;
+    k1 = begin;
   }
 }
 

@@ -36,7 +36,7 @@ struct GradTable {
 
 // Partial sums of a launch: one per block, or with per-tensor sums one per
 // (block, tensor) that meet, at slot block + tensor.
-constexpr int GRAD_MAX_GRID = 148 * 8;
+constexpr int GRAD_MAX_GRID = 148 * 4;
 constexpr uint32_t GRAD_CHUNK_BYTES = 16384;
 
 struct GradNormOut {
