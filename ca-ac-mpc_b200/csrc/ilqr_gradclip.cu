@@ -18,13 +18,14 @@
 #include <cuda_fp16.h>
 
 #include "ilqr_b200.h"
+#include "ilqr_device.cuh"
 #include "ilqr_gradclip.h"
 
 namespace ilqr {
 
 namespace {
 
-constexpr int NT = 256;  // threads of a block
+constexpr int BLK = 256;  // threads of a block
 constexpr int UN = 4;    // 16-byte loads that a thread has in flight
 
 // ---- values ----------------------------------------------------------------
@@ -267,10 +268,10 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   }
   p += h * SZ + tid * 16;
   int64_t left = (n - h) / VE - tid;  // vectors from this thread's first on
-  for (; left > (UN - 1) * NT; left -= UN * NT, p += UN * NT * 16) {
+  for (; left > (UN - 1) * BLK; left -= UN * BLK, p += UN * BLK * 16) {
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * NT * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * BLK * 16);
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
   if (left > 0) {
@@ -278,7 +279,7 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       v[u].w = make_uint4(0, 0, 0, 0);
-      if (left > u * NT) v[u] = load_vec<16>(p + u * NT * 16);
+      if (left > u * BLK) v[u] = load_vec<16>(p + u * BLK * 16);
     }
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
@@ -296,7 +297,7 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
   }
   // from the end: what the sums read last is still in L2
-  const int64_t nv = (n - h) / VE, full = nv / (UN * NT) * (UN * NT);
+  const int64_t nv = (n - h) / VE, full = nv / (UN * BLK) * (UN * BLK);
   int64_t left = nv - full - tid;
   p += h * SZ + (full + tid) * 16;
   q += h * SZ + (full + tid) * 16;
@@ -304,19 +305,19 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * NT) v[u] = load_vec<16>(p + u * NT * 16);
+      if (left > u * BLK) v[u] = load_vec<16>(p + u * BLK * 16);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * NT) *reinterpret_cast<Vec<16>*>(q + u * NT * 16) = scale_vec<DT, 16, false>(v[u], c);
+      if (left > u * BLK) *reinterpret_cast<Vec<16>*>(q + u * BLK * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
-  for (left = full; left > 0; left -= UN * NT) {
-    p -= UN * NT * 16;
-    q -= UN * NT * 16;
+  for (left = full; left > 0; left -= UN * BLK) {
+    p -= UN * BLK * 16;
+    q -= UN * BLK * 16;
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * NT * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * BLK * 16);
 #pragma unroll
-    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * NT * 16) = scale_vec<DT, 16, false>(v[u], c);
+    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * BLK * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
 }
 
@@ -366,7 +367,7 @@ __device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const voi
 __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p, char* q, int64_t n, const Coef& c) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
 #pragma unroll 1
-  for (int64_t i = threadIdx.x; i < n; i += NT) {
+  for (int64_t i = threadIdx.x; i < n; i += BLK) {
     const char* from = p + i * sz;
     float x = dtype == ILQR_DTYPE_F32    ? load_one<ILQR_DTYPE_F32>(from)
               : dtype == ILQR_DTYPE_BF16 ? load_one<ILQR_DTYPE_BF16>(from)
@@ -396,7 +397,7 @@ __device__ __forceinline__ void entry_scale(uint32_t dtype, const void* in, void
 // neighbours, and where a block ends with its tensor the one slot that falls
 // out is set to 0, the identity of both joins.
 template <int CAP, bool MAX, bool PER>
-__global__ void __launch_bounds__(NT) grad_sum_kernel(const __grid_constant__ GradTable<CAP> tab, double* slots) {
+__global__ void __launch_bounds__(BLK) grad_sum_kernel(const __grid_constant__ GradTable<CAP> tab, double* slots) {
   __shared__ double sh[32];
   asm volatile("griddepcontrol.launch_dependents;");
   uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
@@ -431,7 +432,7 @@ __device__ __forceinline__ double join_slots(const double* slots, int64_t n, dou
 
 // Block 0: the norm of the whole list. The others: a warp for each tensor.
 template <int CAP, bool MAX>
-__global__ void __launch_bounds__(NT) grad_join_kernel(const __grid_constant__ GradTable<CAP> tab, uint32_t grid,
+__global__ void __launch_bounds__(BLK) grad_join_kernel(const __grid_constant__ GradTable<CAP> tab, uint32_t grid,
                                                        const double* tab_slots, const double* slots, int64_t n_slots,
                                                        GradNormOut out, int want_global) {
   __shared__ double sh[32];
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(NT) grad_join_kernel(const __grid_constant__ G
     }
     return;
   }
-  const int t = (int)(blockIdx.x - 1) * (NT / 32) + (int)(threadIdx.x >> 5);
+  const int t = (int)(blockIdx.x - 1) * (BLK / 32) + (int)(threadIdx.x >> 5);
   if (t >= tab.n) return;
   const uint32_t c0 = tab.e[t].chunk0, c1 = t + 1 < tab.n ? tab.e[t + 1].chunk0 : tab.chunks;
   const uint32_t lo = block_of(c0, tab.chunks, grid) + t, hi = block_of(c1 - 1, tab.chunks, grid) + t;
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(NT) grad_join_kernel(const __grid_constant__ G
 // out = c in over the list; every block joins the partial sums for itself, in
 // the same order. In place a coefficient of 1 leaves the values where they are.
 template <int CAP>
-__global__ void __launch_bounds__(NT, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
+__global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
                                                         const double* slots, int64_t n_slots, float* norm) {
   __shared__ double sh[32];
   const uint32_t k0 = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
@@ -503,19 +504,142 @@ __device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
   }
 }
 
-// The three steps of a slice. Each thread copies, adds and scales the same
-// vectors: no thread reads what another copied, so the copies need no barrier.
+// How a slice gets to shared memory and back. Long segments move by bulk
+// copies, one each, issued by the lanes of one warp: each segment has a place of
+// whole 16-byte words, lies there at its address modulo 16, and the copy takes
+// its whole words. What is left at its two ends moves value by value, and zeros
+// fill the place, so that sums and products run over whole words. Other slices
+// move by the threads, a vector each.
+struct Piece {
+  uint32_t off;    // of the segment in its place: its address modulo 16
+  uint32_t lead;   // bytes before the first whole word
+  uint32_t whole;  // bytes of whole words
+};
+
+__device__ __forceinline__ Piece piece_of(const RowTensor& r, const char* p) {
+  Piece c;
+  c.off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u);
+  c.lead = -c.off & 15u;
+  c.whole = (r.seg_bytes - c.lead) & ~15u;
+  return c;
+}
+
+// Returns the bytes that this lane's copies bring.
+__device__ __forceinline__ uint32_t bulk_in(const RowTensor& r, int64_t b, uint32_t to, uint64_t* bar, uint32_t lane,
+                                            uint32_t lanes) {
+  const char* p = r.in + b * r.in_row;
+  uint32_t bytes = 0;
+  for (uint32_t s = lane; s < r.n_seg; s += lanes) {
+    const char* from = p + s * r.in_seg;
+    const Piece c = piece_of(r, from);
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            to + s * r.place + c.off + c.lead),
+        "l"(from + c.lead), "r"(c.whole), "r"(smem_u32(bar))
+        : "memory");
+    bytes += c.whole;
+  }
+  return bytes;
+}
+
+__device__ __forceinline__ void bulk_out(const RowTensor& r, int64_t b, uint32_t at, uint32_t lane, uint32_t lanes) {
+  char* q = r.out + b * r.out_row;
+  for (uint32_t s = lane; s < r.n_seg; s += lanes) {
+    char* to = q + s * r.out_seg;
+    const Piece c = piece_of(r, to);
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + c.lead),
+                 "r"(at + s * r.place + c.off + c.lead), "r"(c.whole)
+                 : "memory");
+  }
+}
+
+// The ends of the segments: the first word of a place and the last three hold
+// all that the bulk copies leave.
+template <int VB, bool OUT>
+__device__ __forceinline__ void ends(const RowTensor& r, int64_t b, char* staged, uint32_t lane, uint32_t step) {
+  constexpr uint32_t PER = 64 / VB;
+  char* g = OUT ? r.out + b * r.out_row : const_cast<char*>(r.in) + b * r.in_row;
+  const int64_t seg = OUT ? r.out_seg : r.in_seg;
+  for (uint32_t i = lane; i < r.n_seg * PER; i += step) {
+    const uint32_t s = i / PER, u = (i % PER) * VB;
+    char* q = g + s * seg;
+    const Piece c = piece_of(r, q);
+    const uint32_t at = u < 16 ? u : r.place - 64 + u;
+    if (at - (c.off + c.lead) < c.whole) continue;
+    const bool inside = at - c.off < r.seg_bytes;
+    Vec<VB>* mine = reinterpret_cast<Vec<VB>*>(staged + s * r.place + at);
+    Vec<VB>* theirs = reinterpret_cast<Vec<VB>*>(q + (int64_t)at - c.off);
+    if constexpr (OUT) {
+      if (inside) *theirs = *mine;
+    } else {
+      *mine = inside ? *theirs : Vec<VB>{};
+    }
+  }
+}
+
+template <bool OUT>
+__device__ __forceinline__ void ends(const RowTensor& r, int64_t b, char* staged, uint32_t lane, uint32_t step) {
+  if (r.vec_bytes == 8) ends<8, OUT>(r, b, staged, lane, step);
+  else if (r.vec_bytes == 4) ends<4, OUT>(r, b, staged, lane, step);
+  else ends<2, OUT>(r, b, staged, lane, step);
+}
+
 template <int VB>
-__device__ __forceinline__ void row_copy(const RowTensor& r, int64_t b, uint32_t to, uint32_t lane, uint32_t step) {
+__device__ __forceinline__ void threads_in(const RowTensor& r, int64_t b, uint32_t to, uint32_t lane, uint32_t step) {
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
-#pragma unroll 4
   for (uint32_t i = lane; i < n; i += step) copy_async<VB>(to + i * VB, p + vec_at(r, i, VB, r.in_seg));
 }
 
-template <int DT, int VB, bool STAGED>
-__device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, const char* staged, uint32_t lane,
-                                        uint32_t step) {
+template <int VB>
+__device__ __forceinline__ void threads_out(const RowTensor& r, int64_t b, const char* from, uint32_t lane,
+                                            uint32_t step) {
+  char* q = r.out + b * r.out_row;
+  const uint32_t n = r.n_seg * r.seg_vecs;
+  for (uint32_t i = lane; i < n; i += step)
+    *reinterpret_cast<Vec<VB>*>(q + vec_at(r, i, VB, r.out_seg)) = load_vec<VB>(from + i * VB);
+}
+
+// n 16-byte vectors of shared memory into a sum, and scaled where they are
+template <int DT>
+__device__ __forceinline__ void staged_sum(Acc<false>& a, const char* p, uint32_t n, uint32_t lane, uint32_t step) {
+  for (uint32_t i = lane; i < n; i += UN * step) {
+    Vec<16> v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      v[u] = Vec<16>{};
+      if (i + u * step < n) v[u] = load_vec<16>(p + (i + u * step) * 16);
+    }
+    add_vecs<DT, 16, UN, false>(a, v);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void staged_scale(char* p, uint32_t n, const Coef& c, uint32_t lane, uint32_t step) {
+#pragma unroll 4
+  for (uint32_t i = lane; i < n; i += step) {
+    Vec<16>* v = reinterpret_cast<Vec<16>*>(p + i * 16);
+    *v = scale_vec<DT, 16, false>(*v, c);
+  }
+}
+
+__device__ __forceinline__ void staged_sum(Acc<false>& a, uint32_t dtype, const char* p, uint32_t n, uint32_t lane,
+                                           uint32_t step) {
+  if (dtype == ILQR_DTYPE_F32) staged_sum<ILQR_DTYPE_F32>(a, p, n, lane, step);
+  else if (dtype == ILQR_DTYPE_BF16) staged_sum<ILQR_DTYPE_BF16>(a, p, n, lane, step);
+  else staged_sum<ILQR_DTYPE_F16>(a, p, n, lane, step);
+}
+
+__device__ __forceinline__ void staged_scale(uint32_t dtype, char* p, uint32_t n, const Coef& c, uint32_t lane,
+                                             uint32_t step) {
+  if (dtype == ILQR_DTYPE_F32) staged_scale<ILQR_DTYPE_F32>(p, n, c, lane, step);
+  else if (dtype == ILQR_DTYPE_BF16) staged_scale<ILQR_DTYPE_BF16>(p, n, c, lane, step);
+  else staged_scale<ILQR_DTYPE_F16>(p, n, c, lane, step);
+}
+
+// The same from global memory, for slices that shared memory cannot hold.
+template <int DT, int VB>
+__device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, uint32_t lane, uint32_t step) {
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
   for (uint32_t i = lane; i < n; i += UN * step) {
@@ -524,21 +648,20 @@ __device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64
     for (int u = 0; u < UN; ++u) {
       const uint32_t k = i + u * step;
       v[u] = Vec<VB>{};
-      if (k < n) v[u] = load_vec<VB>(STAGED ? staged + k * VB : p + vec_at(r, k, VB, r.in_seg));
+      if (k < n) v[u] = load_vec<VB>(p + vec_at(r, k, VB, r.in_seg));
     }
     add_vecs<DT, VB, UN, false>(a, v);
   }
 }
 
-template <int DT, int VB, bool STAGED>
-__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const char* staged, const Coef& c,
-                                          uint32_t lane, uint32_t step) {
+template <int DT, int VB>
+__device__ __forceinline__ void row_scale(const RowTensor& r, int64_t b, const Coef& c, uint32_t lane, uint32_t step) {
   const char* p = r.in + b * r.in_row;
   char* q = r.out + b * r.out_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
 #pragma unroll 4
   for (uint32_t i = lane; i < n; i += step) {
-    const Vec<VB> v = load_vec<VB>(STAGED ? staged + i * VB : p + vec_at(r, i, VB, r.in_seg));
+    const Vec<VB> v = load_vec<VB>(p + vec_at(r, i, VB, r.in_seg));
     *reinterpret_cast<Vec<VB>*>(q + vec_at(r, i, VB, r.out_seg)) = scale_vec<DT, VB, false>(v, c);
   }
 }
@@ -582,37 +705,219 @@ __device__ __noinline__ void row_apart(const RowTensor& r, int64_t b, const Coef
     default: CALL(ILQR_DTYPE_BF16, 2); break;                                       \
   }
 
-// G threads (a warp or the block) for each element. STAGED: its slices are
-// copied to shared memory, read from there twice and written once, so global
-// memory is read once; without, both passes read global memory.
-template <int G, int THREADS, bool STAGED>
+// The threads of a group: a part of a warp, a warp, or the block.
+template <int G>
+__device__ __forceinline__ uint32_t group_mask() {
+  if constexpr (G >= 32) return 0xffffffffu;
+  else return ((1u << G) - 1u) << (threadIdx.x % 32 / G * G);
+}
+
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (G <= 32) __syncwarp(group_mask<G>());
+  else __syncthreads();
+}
+
+template <int G>
+__device__ __forceinline__ double group_sum(double v, double* sh) {
+  if constexpr (G > 32) {
+    return block_join<false>(v, sh);
+  } else {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(group_mask<G>(), v, o);
+    return v;
+  }
+}
+
+// The part of a slice that one of several blocks takes: segments, or of a
+// single segment a run of whole 16-byte words.
+__device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, uint32_t parts) {
+  RowTensor x = r;
+  if (r.n_seg > 1) {
+    const uint32_t s0 = (uint32_t)((uint64_t)r.n_seg * rank / parts);
+    const uint32_t s1 = (uint32_t)((uint64_t)r.n_seg * (rank + 1) / parts);
+    x.in += s0 * r.in_seg;
+    x.out += s0 * r.out_seg;
+    x.n_seg = s1 - s0;
+  } else {
+    const uint32_t words = (r.seg_bytes + 15) / 16;
+    const uint32_t o0 = (uint32_t)((uint64_t)words * rank / parts) * 16;
+    const uint32_t o1 = min((uint32_t)((uint64_t)words * (rank + 1) / parts) * 16, r.seg_bytes);
+    x.in += o0;
+    x.out += o0;
+    x.seg_bytes = o1 - o0;
+    x.seg_vecs = x.seg_bytes / r.vec_bytes;
+    x.n_seg = x.seg_bytes > 0 ? 1 : 0;
+    x.place = x.seg_bytes;
+    if (r.bulk == ROW_BULK_ENDS) x.place = (x.seg_bytes + 30) / 16 * 16;
+    if (x.seg_bytes < GRAD_MIN_BULK) x.bulk = ROW_THREADS, x.place = x.seg_bytes;
+  }
+  x.staged_vecs = (x.n_seg * x.place + 15) / 16;
+  return x;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The sum of one value of each block of a cluster, in the order of their ranks.
+// Ends with an arrival that the caller has to wait for before it returns.
+__device__ __forceinline__ double cluster_sum(double v, double* mine) {
+  if (threadIdx.x == 0) *mine = v;
+  cluster_arrive();
+  cluster_wait();
+  double sum = 0.0;
+  for (uint32_t k = 0, n = cluster_size(); k < n; ++k) {
+    uint32_t at;
+    double x;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(k));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
+    sum += x;
+  }
+  cluster_arrive();
+  return sum;
+}
+
+// G threads for each element, whose slices are staged in shared memory: global
+// memory is read once and written once. CLUSTER: the blocks of a cluster share
+// one element.
+template <int G, int THREADS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constant__ RowTable tab) {
   extern __shared__ __align__(16) char staged[];
-  __shared__ double sh[32];
+  __shared__ double sh[33];
+  __shared__ uint64_t bars[THREADS / G];
+  __shared__ RowTensor parts[CLUSTER ? ROW_MAX_TENSORS : 1];
   constexpr int PER = THREADS / G;
-  const int64_t b = PER == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * PER + threadIdx.x / G;
-  if (b >= tab.B) return;  // of a whole warp, or not at all
-  const uint32_t lane = threadIdx.x % G;
-  const char* mine = staged + (PER == 1 ? 0 : (threadIdx.x / G) * tab.staged_bytes);
-  if (STAGED) {
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine);
-    for (int k = 0; k < tab.n; ++k) {
-      const RowTensor& r = tab.t[k];
-      if (r.vec_bytes == 16) row_copy<16>(r, b, to + r.staged, lane, G);
-      else if (r.vec_bytes == 8) row_copy<8>(r, b, to + r.staged, lane, G);
-      else if (r.vec_bytes == 4) row_copy<4>(r, b, to + r.staged, lane, G);
-      else row_copy<2>(r, b, to + r.staged, lane, G);
+  constexpr uint32_t LANES = G < 32 ? G : 32;  // that issue bulk copies
+  const uint32_t group = threadIdx.x / G, lane = threadIdx.x % G;
+  int64_t b = (int64_t)blockIdx.x * PER + group;
+  uint32_t staged_bytes = tab.staged_bytes;
+  const RowTensor* tensors = tab.t;
+  if constexpr (CLUSTER) {
+    const uint32_t rank = cluster_rank(), n = cluster_size();
+    b = blockIdx.x / n;
+    if (threadIdx.x < tab.n) parts[threadIdx.x] = part_of(tab.t[threadIdx.x], rank, n);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t at = 0;
+      for (int k = 0; k < tab.n; ++k) {
+        parts[k].staged = at;
+        at += parts[k].staged_vecs * 16;
+      }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    tensors = parts;
+    staged_bytes = parts[tab.n - 1].staged + parts[tab.n - 1].staged_vecs * 16;
   }
+  if (b >= tab.B) return;  // of a whole group, or not at all
+  char* mine = staged + group * staged_bytes;
+  const uint32_t to = smem_u32(mine);
+  uint64_t* bar = bars + group;
+  if (tab.bulk && lane < LANES) {
+    if (lane == 0) {
+      mbar_init(bar, LANES);
+      fence_mbar_init();
+    }
+    __syncwarp(group_mask<G>());
+    uint32_t bytes = 0;
+    for (int k = 0; k < tab.n; ++k)
+      if (tensors[k].bulk) bytes += bulk_in(tensors[k], b, to + tensors[k].staged, bar, lane, LANES);
+    mbar_expect_tx(bar, bytes);
+  }
+  for (int k = 0; k < tab.n; ++k) {
+    const RowTensor& r = tensors[k];
+    if (r.bulk) {
+      if (r.bulk == ROW_BULK_ENDS) ends<false>(r, b, mine + r.staged, lane, G);
+      continue;
+    }
+    if (r.vec_bytes == 16) threads_in<16>(r, b, to + r.staged, lane, G);
+    else if (r.vec_bytes == 8) threads_in<8>(r, b, to + r.staged, lane, G);
+    else if (r.vec_bytes == 4) threads_in<4>(r, b, to + r.staged, lane, G);
+    else threads_in<2>(r, b, to + r.staged, lane, G);
+    // zeros after it, to a whole word
+    const uint32_t end = r.n_seg * r.seg_bytes;
+    if (lane < (-end & 15u) / 2) *reinterpret_cast<uint16_t*>(mine + r.staged + end + 2 * lane) = 0;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  group_sync<G>();  // the threads' copies and the barrier's set-up
+  Acc<false> a;
+  // copies that never come (after a second, as bounded, wait) make the
+  // element's norm NaN
+  if (tab.bulk && !mbar_wait(bar, 0) && !mbar_wait(bar, 0)) a.s = __longlong_as_double(0x7ff8000000000000ll);
+  if (tab.one_dtype) {
+    staged_sum(a, tab.t[0].dtype, mine, staged_bytes / 16, lane, G);
+  } else {
+    for (int k = 0; k < tab.n; ++k)
+      staged_sum(a, tensors[k].dtype, mine + tensors[k].staged, tensors[k].staged_vecs, lane, G);
+  }
+  double total = group_sum<G>(a.s, sh);
+  if constexpr (CLUSTER) total = cluster_sum(total, sh + 32);
+  const double nrm = sqrt(total);
+  if (lane == 0 && tab.norms != nullptr && (!CLUSTER || cluster_rank() == 0)) tab.norms[b] = (float)nrm;
+  const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
+  const bool zero = tab.zero_nonfinite && !isfinite(nrm);
+  if (zero || c.wide) {
+    for (int k = 0; k < tab.n; ++k) row_apart(tensors[k], b, c, zero, lane, G);
+    if constexpr (CLUSTER) cluster_wait();
+    return;
+  }
+  if (c.d != 1.0) {
+    if (tab.one_dtype) {
+      staged_scale(tab.t[0].dtype, mine, staged_bytes / 16, c, lane, G);
+    } else {
+      for (int k = 0; k < tab.n; ++k)
+        staged_scale(tensors[k].dtype, mine + tensors[k].staged, tensors[k].staged_vecs, c, lane, G);
+    }
+    fence_proxy_async();
+    group_sync<G>();
+  }
+  if (tab.bulk && lane < LANES) {
+    for (int k = 0; k < tab.n; ++k) {
+      const RowTensor& r = tensors[k];
+      if (r.bulk && !(c.d == 1.0 && r.in == r.out)) bulk_out(r, b, to + r.staged, lane, LANES);
+    }
+    bulk_commit();
+  }
+  for (int k = 0; k < tab.n; ++k) {
+    const RowTensor& r = tensors[k];
+    if (c.d == 1.0 && r.in == r.out) continue;
+    if (r.bulk) {
+      if (r.bulk == ROW_BULK_ENDS) ends<true>(r, b, mine + r.staged, lane, G);
+      continue;
+    }
+    if (r.vec_bytes == 16) threads_out<16>(r, b, mine + r.staged, lane, G);
+    else if (r.vec_bytes == 8) threads_out<8>(r, b, mine + r.staged, lane, G);
+    else if (r.vec_bytes == 4) threads_out<4>(r, b, mine + r.staged, lane, G);
+    else threads_out<2>(r, b, mine + r.staged, lane, G);
+  }
+  if (tab.bulk && lane < LANES) bulk_wait_read<0>();  // the copies read this block's memory
+  if constexpr (CLUSTER) cluster_wait();              // and the cluster's blocks their sums
+}
+
+// Elements that shared memory cannot hold: both passes read global memory.
+__global__ void __launch_bounds__(BLK) grad_long_rows_kernel(const __grid_constant__ RowTable tab) {
+  __shared__ double sh[32];
+  const int64_t b = blockIdx.x;
+  const uint32_t lane = threadIdx.x;
   Acc<false> a;
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tab.t[k];
-#define CALL(DT, VB) row_sum<DT, VB, STAGED>(a, r, b, mine + r.staged, lane, G)
+#define CALL(DT, VB) row_sum<DT, VB>(a, r, b, lane, BLK)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
-  const double nrm = sqrt(G == 32 ? warp_join<false>(a.s) : block_join<false>(a.s, sh));
+  const double nrm = sqrt(block_join<false>(a.s, sh));
   if (lane == 0 && tab.norms != nullptr) tab.norms[b] = (float)nrm;
   const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
   const bool zero = tab.zero_nonfinite && !isfinite(nrm);
@@ -620,10 +925,10 @@ __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constan
     const RowTensor& r = tab.t[k];
     if (c.d == 1.0 && !zero && r.in == r.out) continue;
     if (zero || c.wide) {
-      row_apart(r, b, c, zero, lane, G);
+      row_apart(r, b, c, zero, lane, BLK);
       continue;
     }
-#define CALL(DT, VB) row_scale<DT, VB, STAGED>(r, b, mine + r.staged, c, lane, G)
+#define CALL(DT, VB) row_scale<DT, VB>(r, b, c, lane, BLK)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
@@ -635,7 +940,7 @@ template <typename... K, typename... A>
 cudaError_t launch(void (*kernel)(K...), unsigned grid, bool dependent, cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(NT);
+  cfg.blockDim = dim3(BLK);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -662,7 +967,7 @@ cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* 
                              const double* slots, int64_t n_slots, const GradNormOut& out, bool want_global,
                              cudaStream_t stream) {
   static const GradTable<CAP> none{};
-  const unsigned blocks = 1 + (tab != nullptr ? (unsigned)(tab->n + NT / 32 - 1) / (NT / 32) : 0);
+  const unsigned blocks = 1 + (tab != nullptr ? (unsigned)(tab->n + BLK / 32 - 1) / (BLK / 32) : 0);
   const GradTable<CAP>& use = tab != nullptr ? *tab : none;
   return max_type ? launch(grad_join_kernel<CAP, true>, blocks, true, stream, use, (uint32_t)grid, tab_slots, slots,
                            n_slots, out, want_global ? 1 : 0)
@@ -688,30 +993,61 @@ INSTANTIATE(GRAD_CAP_LONG)
 
 namespace {
 
-template <int G, int THREADS, bool STAGED>
-cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream) {
-  constexpr int PER = THREADS / G;
-  const size_t smem = STAGED ? (size_t)tab.staged_bytes * PER : 0;
-  const auto kernel = grad_rows_kernel<G, THREADS, STAGED>;
-  if (STAGED) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+// The most that one of `parts` blocks stages of an element: up to a segment and
+// the words' ends of each tensor beyond the even share.
+size_t part_bytes(const RowTable& tab, size_t parts) {
+  size_t bytes = 0;
+  for (int k = 0; k < tab.n; ++k) {
+    const RowTensor& r = tab.t[k];
+    bytes += r.n_seg > 1 ? ((r.n_seg + parts - 1) / parts * r.place + 15) / 16 * 16
+                         : (r.staged_vecs + parts - 1) / parts * 16 + 48;
   }
+  return bytes;
+}
+
+template <int G, int THREADS, bool CLUSTER = false>
+cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned cluster = 1) {
+  constexpr int PER = THREADS / G;
+  const size_t smem = CLUSTER ? part_bytes(tab, cluster) : (size_t)tab.staged_bytes * PER;
+  const auto kernel = grad_rows_kernel<G, THREADS, CLUSTER>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((tab.B + PER - 1) / PER));
+  cfg.gridDim = dim3((unsigned)((tab.B + PER - 1) / PER) * cluster);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {cluster, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, tab);
 }
 
 }  // namespace
 
 cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
-  if (tab.staged_bytes <= 4096) return launch_rows<32, 128, true>(tab, stream);
-  if (tab.staged_bytes <= 20480) return launch_rows<128, 128, true>(tab, stream);
-  if (tab.staged_bytes <= 220000) return launch_rows<256, 256, true>(tab, stream);
-  return launch_rows<256, 256, false>(tab, stream);
+  // Threads for an element by what it stages. More threads cost instructions
+  // that every element repeats (its records, the join, square root and quotient),
+  // fewer leave the additions of long elements to few: us at 8 | 32 | 64 | 128
+  // threads, by bytes of an element (number of elements):
+  //   266 (100000)  19 | 58 | 122 | 212     8442 (16384)   82 | 49 | 52 | 72
+  //  1722 (40000)   26 | 41 |  78 | 128    16842 (16384)   -- | 87 | 87 | 86
+  //  2280 (16384)   23 | 18 |  26 |  41    24534 (4096)    -- | 64 | 53 | 49
+  //  5642 (16384)   38 | 31 |  33 |  46    42042 (65536)   -- | 1030 | 930 | 880
+  if (tab.staged_bytes <= 2048) return launch_rows<8, 128>(tab, stream);
+  if (tab.staged_bytes <= 12288) return launch_rows<32, 128>(tab, stream);
+  if (tab.staged_bytes <= 20480) return launch_rows<64, 64>(tab, stream);
+  if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream);
+  // Longer ones leave an SM one or two blocks, whose copies, sums and stores
+  // take turns: blocks of a cluster share them. us in one block | 2 | 4 | 8:
+  //  84042 (2048)  91 | 82 | 92 | 137      210042 (1024)  162 | 126 | 110 | 108
+  if (tab.B <= INT32_MAX / 8)
+    for (unsigned parts = 2; parts <= 8; parts *= 2)
+      if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
+        return launch_rows<128, 128, true>(tab, stream, parts);
+  return launch(grad_long_rows_kernel, (unsigned)tab.B, false, stream, tab);
 }
 
 }  // namespace ilqr

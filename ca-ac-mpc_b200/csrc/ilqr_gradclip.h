@@ -61,8 +61,16 @@ struct RowTensor {
   uint32_t vec_bytes, dtype;
   uint32_t magic, shift;  // i / seg_vecs = i magic >> (32 + shift)
   uint32_t staged;        // where the slice is staged, from the element's place
+  uint32_t staged_vecs;   // 16-byte words that it takes there
+  uint32_t seg_bytes;
+  uint32_t place;         // bytes from one staged segment to the next
+  uint32_t bulk;          // what moves it
   uint32_t pad;
 };
+
+constexpr uint32_t ROW_THREADS = 0;    // the threads, a vector each
+constexpr uint32_t ROW_BULK = 1;       // bulk copies: its segments are whole 16-byte words
+constexpr uint32_t ROW_BULK_ENDS = 2;  // bulk copies, and the threads at the segments' ends
 
 constexpr int ROW_MAX_TENSORS = 8;
 
@@ -74,8 +82,15 @@ struct RowTable {
   double max_norm, eps;
   float* norms;
   uint32_t staged_bytes;  // of an element, every slice from a multiple of 16
+  uint32_t bulk;          // whether bulk copies move any of it
+  uint32_t one_dtype;
   uint32_t pad;
 };
+
+// Of the 227 KB of shared memory that a block can have.
+constexpr uint32_t GRAD_MAX_STAGED = 224 * 1024;
+// Segments from this many bytes on move by bulk copies.
+constexpr uint32_t GRAD_MIN_BULK = 256;
 
 template <int CAP>
 cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, bool per_tensor, double* slots,

@@ -297,6 +297,7 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
   std::memset(&tab, 0, sizeof(tab));
   Rows ins[ILQR_MAX_ELEMENT_TENSORS], outs[ILQR_MAX_ELEMENT_TENSORS];
   int64_t row_bytes = 0;
+  tab.one_dtype = 1;
   for (int32_t i = 0; i < n_tensors; ++i) {
     const int64_t* g = layout + 6 * i;
     const int64_t n_seg = g[0], len = g[1];
@@ -332,7 +333,22 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
     r.vec_bytes = vec, r.dtype = (uint32_t)dtypes[i];
     reciprocal(r.seg_vecs, &r.magic, &r.shift);
     r.staged = (uint32_t)std::min<int64_t>(row_bytes, UINT32_MAX);
-    row_bytes += (n_seg * len * sz + 15) / 16 * 16;
+    r.seg_bytes = (uint32_t)std::min<int64_t>(len * sz, UINT32_MAX);
+    // what every address of the input has in common with the output's
+    uintptr_t off = p ^ q;
+    if (n_seg > 1) off |= (uintptr_t)(ins[k].seg - outs[k].seg);
+    if (B > 1) off |= (uintptr_t)(ins[k].row - outs[k].row);
+    int64_t place = len * sz;
+    if (len * sz >= ilqr::GRAD_MIN_BULK && (off & 15u) == 0) {
+      r.bulk = vec == 16 ? ilqr::ROW_BULK : ilqr::ROW_BULK_ENDS;
+      if (vec != 16) place = (place + 30) / 16 * 16;
+      tab.bulk = 1;
+    }
+    r.place = (uint32_t)std::min<int64_t>(place, UINT32_MAX);
+    const int64_t words = (n_seg * place + 15) / 16;
+    r.staged_vecs = (uint32_t)std::min<int64_t>(words, UINT32_MAX);
+    row_bytes += words * 16;
+    if (r.dtype != tab.t[0].dtype) tab.one_dtype = 0;
   }
   for (int a = 0; a < tab.n; ++a)
     for (int b = 0; b < tab.n; ++b) {

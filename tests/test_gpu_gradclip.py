@@ -371,6 +371,24 @@ def test_elements_of_every_width(width):
     _check_elements([odd[:, 1:], odd[:, :1]], [0, 0], math.sqrt(width), out=[odd[:, 1:], odd[:, :1]])
 
 
+def test_elements_longer_than_shared_memory():
+    """Elements that a cluster's blocks share, and those that no block can hold."""
+    for shape, d in (((3, 90_001), 0), ((2, 500_003), 0), ((2, 3, 300_001), 1), ((61, 3, 5003), 1), ((9, 2, 30_000), 1),
+                     ((5, 1, 70_000), 1), ((1, 300_000), 0)):
+        for dtype in TYPES:
+            x = _values(shape, dtype, 3)
+            y = _values((shape[d], 77), F32, 4)
+            width = x.numel() // shape[d]
+            x.select(d, 0).mul_(0.2)
+            _check_elements([y, x], [0, d], math.sqrt(width) * 0.7)
+            _check_elements([y, x], [0, d], math.sqrt(width) * 0.7, out=[y, x])
+    x = _values((2, 100_000), F32, 5)
+    x[1, 70_000] = math.inf
+    for zero in (False, True):
+        _check_elements([x], [0], 3.0, zero=zero)
+    _check_elements([x[:1]], [0], 1e-36)             # a coefficient below the floats' range
+
+
 def test_elements_of_other_layouts():
     B = 9
     x = _values((4, B, 3, 5), F32, 1)
