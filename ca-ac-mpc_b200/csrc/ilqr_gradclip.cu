@@ -14,6 +14,8 @@
 // group's sum is under 2^-100) are formed again in 64 bits, so a norm is right
 // wherever it is a float itself. The order of every sum is fixed by sizes and
 // grid: no atomics, the same bits each time.
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -161,6 +163,42 @@ __device__ __forceinline__ double block_join(double v, double* sh) {
   return warp_join<MAX>(v);
 }
 
+// ---- clusters ---------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The join of one value of each block of a cluster, in the order of their
+// ranks. Ends with an arrival that the caller has to wait for before it returns.
+template <bool MAX>
+__device__ __forceinline__ double cluster_join(double v, double* mine) {
+  if (threadIdx.x == 0) *mine = v;
+  cluster_arrive();
+  cluster_wait();
+  double all = 0.0;
+  for (uint32_t k = 0, n = cluster_size(); k < n; ++k) {
+    uint32_t at;
+    double x;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(k));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
+    all = join<MAX>(all, x);
+  }
+  cluster_arrive();
+  return all;
+}
+
 __device__ __forceinline__ double norm_of(double total, bool max_type) { return max_type ? total : sqrt(total); }
 
 // WIDE: the coefficient is so small that as a float it has lost bits; the
@@ -256,7 +294,7 @@ __device__ __forceinline__ int head_of(const char* p, int64_t n) {
   return n < h ? (int)n : h;
 }
 
-template <int DT, bool MAX>
+template <int DT, bool MAX, int THREADS>
 __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
   const int tid = threadIdx.x;
@@ -268,10 +306,10 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   }
   p += h * SZ + tid * 16;
   int64_t left = (n - h) / VE - tid;  // vectors from this thread's first on
-  for (; left > (UN - 1) * BLK; left -= UN * BLK, p += UN * BLK * 16) {
+  for (; left > (UN - 1) * THREADS; left -= UN * THREADS, p += UN * THREADS * 16) {
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * BLK * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * THREADS * 16);
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
   if (left > 0) {
@@ -279,14 +317,14 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       v[u].w = make_uint4(0, 0, 0, 0);
-      if (left > u * BLK) v[u] = load_vec<16>(p + u * BLK * 16);
+      if (left > u * THREADS) v[u] = load_vec<16>(p + u * THREADS * 16);
     }
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
 }
 
 // out = c in; `in` may be `out`
-template <int DT>
+template <int DT, int THREADS>
 __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
   const int tid = threadIdx.x;
@@ -297,7 +335,7 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
   }
   // from the end: what the sums read last is still in L2
-  const int64_t nv = (n - h) / VE, full = nv / (UN * BLK) * (UN * BLK);
+  const int64_t nv = (n - h) / VE, full = nv / (UN * THREADS) * (UN * THREADS);
   int64_t left = nv - full - tid;
   p += h * SZ + (full + tid) * 16;
   q += h * SZ + (full + tid) * 16;
@@ -305,19 +343,19 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * BLK) v[u] = load_vec<16>(p + u * BLK * 16);
+      if (left > u * THREADS) v[u] = load_vec<16>(p + u * THREADS * 16);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * BLK) *reinterpret_cast<Vec<16>*>(q + u * BLK * 16) = scale_vec<DT, 16, false>(v[u], c);
+      if (left > u * THREADS) *reinterpret_cast<Vec<16>*>(q + u * THREADS * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
-  for (left = full; left > 0; left -= UN * BLK) {
-    p -= UN * BLK * 16;
-    q -= UN * BLK * 16;
+  for (left = full; left > 0; left -= UN * THREADS) {
+    p -= UN * THREADS * 16;
+    q -= UN * THREADS * 16;
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * BLK * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * THREADS * 16);
 #pragma unroll
-    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * BLK * 16) = scale_vec<DT, 16, false>(v[u], c);
+    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * THREADS * 16) = scale_vec<DT, 16, false>(v[u], c);
   }
 }
 
@@ -354,20 +392,21 @@ __device__ __forceinline__ void span(const GradTable<CAP>& tab, int t, uint32_t 
   *n = (b < e.numel ? b : e.numel) - a;
 }
 
-template <bool MAX>
+template <bool MAX, int THREADS>
 __device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const void* in, int64_t at, int64_t n) {
   const char* p = static_cast<const char*>(in);
-  if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX>(a, p + at * 4, n);
-  else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX>(a, p + at * 2, n);
-  else range_sum<ILQR_DTYPE_F16, MAX>(a, p + at * 2, n);
+  if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX, THREADS>(a, p + at * 4, n);
+  else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX, THREADS>(a, p + at * 2, n);
+  else range_sum<ILQR_DTYPE_F16, MAX, THREADS>(a, p + at * 2, n);
 }
 
 // Value by value: for coefficients below the floats' range, and for `in` and
 // `out` that lie differently in their 16-byte words.
+template <int THREADS>
 __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p, char* q, int64_t n, const Coef& c) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
 #pragma unroll 1
-  for (int64_t i = threadIdx.x; i < n; i += BLK) {
+  for (int64_t i = threadIdx.x; i < n; i += THREADS) {
     const char* from = p + i * sz;
     float x = dtype == ILQR_DTYPE_F32    ? load_one<ILQR_DTYPE_F32>(from)
               : dtype == ILQR_DTYPE_BF16 ? load_one<ILQR_DTYPE_BF16>(from)
@@ -380,16 +419,17 @@ __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p,
   }
 }
 
+template <int THREADS>
 __device__ __forceinline__ void entry_scale(uint32_t dtype, const void* in, void* out, int64_t at, int64_t n,
                                             const Coef& c) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
   const char* p = static_cast<const char*>(in) + at * sz;
   char* q = static_cast<char*>(out) + at * sz;
   if (c.wide || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u))
-    entry_scale_apart(dtype, p, q, n, c);
-  else if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32>(p, q, n, c);
-  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16>(p, q, n, c);
-  else range_scale<ILQR_DTYPE_F16>(p, q, n, c);
+    entry_scale_apart<THREADS>(dtype, p, q, n, c);
+  else if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32, THREADS>(p, q, n, c);
+  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16, THREADS>(p, q, n, c);
+  else range_scale<ILQR_DTYPE_F16, THREADS>(p, q, n, c);
 }
 
 // Partial sums. Each block takes a contiguous run of chunks; with PER one sum
@@ -409,7 +449,7 @@ __global__ void __launch_bounds__(BLK) grad_sum_kernel(const __grid_constant__ G
     const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
     int64_t at, n;
     span(tab, t, k, end, &at, &n);
-    entry_sum<MAX>(a, tab.e[t].dtype, tab.e[t].in, at, n);
+    entry_sum<MAX, BLK>(a, tab.e[t].dtype, tab.e[t].in, at, n);
     if (PER) {
       const double v = block_join<MAX>(value(a), sh);
       if (threadIdx.x == 0) slots[blockIdx.x + t] = v;
@@ -456,30 +496,63 @@ __global__ void __launch_bounds__(BLK) grad_join_kernel(const __grid_constant__ 
   if ((threadIdx.x & 31) == 0) out.tensor_norms[t] = (float)norm_of(v, MAX);
 }
 
-// out = c in over the list; every block joins the partial sums for itself, in
-// the same order. In place a coefficient of 1 leaves the values where they are.
-template <int CAP>
-__global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
-                                                        const double* slots, int64_t n_slots, float* norm) {
-  __shared__ double sh[32];
-  const uint32_t k0 = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
-  uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
-  int t = find(tab, k1 - 1);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const double total = s.max_type ? join_slots<true>(slots, n_slots, sh) : join_slots<false>(slots, n_slots, sh);
-  const double nrm = norm_of(total, s.max_type);
-  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
-  const Coef c = coef_of(nrm, s.max_norm, s.eps);
+// out = c in over chunks [k0, k1), from the end. In place a coefficient of 1
+// leaves the values where they are.
+template <int CAP, int THREADS>
+__device__ __forceinline__ void chunks_scale(const GradTable<CAP>& tab, uint32_t k0, uint32_t k1, int t, const Coef& c) {
   for (; k1 > k0; --t) {
     const GradEntry& e = tab.e[t];
     const uint32_t begin = max(k0, e.chunk0);
     if (!(c.d == 1.0 && e.in == e.out)) {
       int64_t at, n;
       span(tab, t, begin, k1, &at, &n);
-      entry_scale(e.dtype, e.in, e.out, at, n, c);
+      entry_scale<THREADS>(e.dtype, e.in, e.out, at, n, c);
     }
     k1 = begin;
   }
+}
+
+// Every block joins the partial sums for itself, in the same order.
+template <int CAP>
+__global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
+                                                            const double* slots, int64_t n_slots, float* norm) {
+  __shared__ double sh[32];
+  const uint32_t k0 = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
+  const uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
+  const int t = find(tab, k1 - 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double total = s.max_type ? join_slots<true>(slots, n_slots, sh) : join_slots<false>(slots, n_slots, sh);
+  const double nrm = norm_of(total, s.max_type);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
+  chunks_scale<CAP, BLK>(tab, k0, k1, t, coef_of(nrm, s.max_norm, s.eps));
+}
+
+// A short list by one cluster, in one launch and without a workspace: the
+// blocks' sums meet in shared memory, and what they read again is in L1 or L2.
+template <int CAP, bool MAX, bool SCALE>
+__global__ void __launch_bounds__(BLK) grad_small_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
+                                                               GradNormOut out) {
+  __shared__ double sh[33];
+  const uint32_t rank = cluster_rank(), n_blocks = cluster_size();
+  const uint32_t k0 = first_chunk(rank, tab.chunks, n_blocks), k1 = first_chunk(rank + 1, tab.chunks, n_blocks);
+  Acc<MAX> a;
+  int t = 0;
+  if (k0 < k1) t = find(tab, k0);
+  for (uint32_t k = k0; k < k1; ++t) {
+    const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
+    int64_t at, n;
+    span(tab, t, k, end, &at, &n);
+    entry_sum<MAX, BLK>(a, tab.e[t].dtype, tab.e[t].in, at, n);
+    k = end;
+  }
+  const double total = cluster_join<MAX>(block_join<MAX>(value(a), sh), sh + 32);
+  const double nrm = norm_of(total, MAX);
+  if (rank == 0 && threadIdx.x == 0) {
+    if (out.norm != nullptr) *out.norm = (float)nrm;
+    if (out.total != nullptr) *out.total = total;
+  }
+  if constexpr (SCALE) chunks_scale<CAP, BLK>(tab, k0, k1, t - 1, coef_of(nrm, s.max_norm, s.eps));
+  cluster_wait();
 }
 
 // ---- batch elements ---------------------------------------------------------
@@ -756,39 +829,6 @@ __device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, 
   return x;
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-
-// The sum of one value of each block of a cluster, in the order of their ranks.
-// Ends with an arrival that the caller has to wait for before it returns.
-__device__ __forceinline__ double cluster_sum(double v, double* mine) {
-  if (threadIdx.x == 0) *mine = v;
-  cluster_arrive();
-  cluster_wait();
-  double sum = 0.0;
-  for (uint32_t k = 0, n = cluster_size(); k < n; ++k) {
-    uint32_t at;
-    double x;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(k));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
-    sum += x;
-  }
-  cluster_arrive();
-  return sum;
-}
-
 // G threads for each element, whose slices are staged in shared memory: global
 // memory is read once and written once. CLUSTER: the blocks of a cluster share
 // one element.
@@ -862,7 +902,7 @@ __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constan
       staged_sum(a, tensors[k].dtype, mine + tensors[k].staged, tensors[k].staged_vecs, lane, G);
   }
   double total = group_sum<G>(a.s, sh);
-  if constexpr (CLUSTER) total = cluster_sum(total, sh + 32);
+  if constexpr (CLUSTER) total = cluster_join<false>(total, sh + 32);
   const double nrm = sqrt(total);
   if (lane == 0 && tab.norms != nullptr && (!CLUSTER || cluster_rank() == 0)) tab.norms[b] = (float)nrm;
   const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
@@ -981,12 +1021,42 @@ cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradSca
   return launch(grad_scale_kernel<CAP>, grid, dependent, stream, tab, s, slots, n_slots, norm);
 }
 
+template <int CAP, bool MAX, bool SCALE>
+static cudaError_t launch_small(const GradTable<CAP>& tab, const GradScale& s, const GradNormOut& out,
+                                cudaStream_t stream) {
+  unsigned blocks = 1;
+  while (blocks < (unsigned)GRAD_SMALL_BLOCKS && blocks < tab.chunks) blocks *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(BLK);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {blocks, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, grad_small_kernel<CAP, MAX, SCALE>, tab, s, out);
+}
+
+template <int CAP>
+cudaError_t launch_grad_small(const GradTable<CAP>& tab, bool max_type, const GradScale* s, const GradNormOut& out,
+                              cudaStream_t stream) {
+  const GradScale none{};
+  if (s != nullptr)
+    return max_type ? launch_small<CAP, true, true>(tab, *s, out, stream)
+                    : launch_small<CAP, false, true>(tab, *s, out, stream);
+  return max_type ? launch_small<CAP, true, false>(tab, none, out, stream)
+                  : launch_small<CAP, false, false>(tab, none, out, stream);
+}
+
 #define INSTANTIATE(CAP)                                                                                              \
   template cudaError_t launch_grad_sum<CAP>(const GradTable<CAP>&, int, bool, bool, double*, cudaStream_t);           \
   template cudaError_t launch_grad_join<CAP>(const GradTable<CAP>*, int, const double*, bool, const double*, int64_t, \
                                              const GradNormOut&, bool, cudaStream_t);                                 \
   template cudaError_t launch_grad_scale<CAP>(const GradTable<CAP>&, int, const GradScale&, const double*, int64_t,   \
                                               float*, bool, cudaStream_t);
+template cudaError_t launch_grad_small<GRAD_CAP_SHORT>(const GradTable<GRAD_CAP_SHORT>&, bool, const GradScale*,
+                                                       const GradNormOut&, cudaStream_t);
 INSTANTIATE(GRAD_CAP_SHORT)
 INSTANTIATE(GRAD_CAP_LONG)
 #undef INSTANTIATE
@@ -1010,8 +1080,16 @@ cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned clust
   constexpr int PER = THREADS / G;
   const size_t smem = CLUSTER ? part_bytes(tab, cluster) : (size_t)tab.staged_bytes * PER;
   const auto kernel = grad_rows_kernel<G, THREADS, CLUSTER>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may have all shared memory
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GRAD_MAX_STAGED);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((tab.B + PER - 1) / PER) * cluster);
   cfg.blockDim = dim3(THREADS);

@@ -39,6 +39,13 @@ struct GradTable {
 constexpr int GRAD_MAX_GRID = 148 * 4;
 constexpr uint32_t GRAD_CHUNK_BYTES = 16384;
 
+// A list up to this size is short: one cluster takes it, in one launch instead
+// of two (two | one, us of GPU time and of an eager call: clipping 128 KB
+// 4.1 | 4.3 and 8.4 | 6.9; 512 KB 4.2 | 6.2 and 8.5 | 8.5).
+constexpr int64_t GRAD_SMALL_BYTES = 128 << 10;
+constexpr uint32_t GRAD_SMALL_CHUNK_BYTES = 4096;
+constexpr int GRAD_SMALL_BLOCKS = 8;
+
 struct GradNormOut {
   float* norm;          // may be null
   float* tensor_norms;  // may be null
@@ -104,6 +111,10 @@ cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* 
 template <int CAP>
 cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
                               int64_t n_slots, float* norm, bool dependent, cudaStream_t stream);
+// A short list in one launch; s == nullptr: its norm only.
+template <int CAP>
+cudaError_t launch_grad_small(const GradTable<CAP>& tab, bool max_type, const GradScale* s, const GradNormOut& out,
+                              cudaStream_t stream);
 cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream);
 
 }  // namespace ilqr

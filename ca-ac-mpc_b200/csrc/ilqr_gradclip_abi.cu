@@ -78,22 +78,31 @@ bool overlaps(const List& l) {
   return false;
 }
 
-uint64_t chunks_of(int64_t numel, int32_t dtype) {
-  const uint64_t c = ((uint64_t)(numel * size_of(dtype)) + ilqr::GRAD_CHUNK_BYTES - 1) / ilqr::GRAD_CHUNK_BYTES;
+uint64_t chunks_of(int64_t numel, int32_t dtype, uint32_t chunk_bytes) {
+  const uint64_t c = ((uint64_t)(numel * size_of(dtype)) + chunk_bytes - 1) / chunk_bytes;
   return c > 0 ? c : 1;
 }
 
+// Whether a list is short enough for the one-launch form.
+bool is_small(const List& l) {
+  if (l.n > ilqr::GRAD_CAP_SHORT) return false;
+  int64_t bytes = 0;
+  for (int32_t i = 0; i < l.n; ++i) bytes += l.numel[i] * size_of(l.dtype[i]);
+  return bytes <= ilqr::GRAD_SMALL_BYTES;
+}
+
 template <int CAP>
-void fill(GradTable<CAP>& tab, const List& l, int32_t first, int32_t n) {
+void fill(GradTable<CAP>& tab, const List& l, int32_t first, int32_t n,
+          uint32_t chunk_bytes = ilqr::GRAD_CHUNK_BYTES) {
   tab.n = n;
-  tab.chunk_bytes = ilqr::GRAD_CHUNK_BYTES;
+  tab.chunk_bytes = chunk_bytes;
   tab.pad = 0;
   uint64_t at = 0;
   for (int32_t i = 0; i < n; ++i) {
     const int32_t k = first + i;
     tab.e[i] = GradEntry{l.in[k], l.out != nullptr ? l.out[k] : nullptr, l.numel[k], (uint32_t)at,
                          (uint32_t)l.dtype[k]};
-    at += chunks_of(l.numel[k], l.dtype[k]);
+    at += chunks_of(l.numel[k], l.dtype[k], chunk_bytes);
   }
   tab.chunks = (uint32_t)at;
 }
@@ -166,6 +175,13 @@ int clip_impl(const List& l, const ilqr::GradScale& s, const double* total, floa
   return ILQR_OK;
 }
 
+int small_impl(const List& l, bool max_type, const ilqr::GradScale* s, const ilqr::GradNormOut& o,
+               cudaStream_t stream) {
+  GradTable<ilqr::GRAD_CAP_SHORT> tab;
+  fill(tab, l, 0, l.n, ilqr::GRAD_SMALL_CHUNK_BYTES);
+  return status_of(ilqr::launch_grad_small(tab, max_type, s, o, stream));
+}
+
 int64_t magnitude(int64_t v) { return v < 0 ? -v : v; }
 
 }  // namespace
@@ -196,6 +212,7 @@ int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const in
     const ilqr::GradNormOut o{norm, tensor_norms, total};
     double* slots = static_cast<double*>(workspace);
     const bool mx = norm_type == ILQR_NORM_MAX;
+    if (tensor_norms == nullptr && is_small(l)) return small_impl(l, mx, nullptr, o, stream);
     return n_tensors <= ilqr::GRAD_CAP_SHORT ? norm_impl<ilqr::GRAD_CAP_SHORT>(l, mx, o, slots, stream)
                                              : norm_impl<ilqr::GRAD_CAP_LONG>(l, mx, o, slots, stream);
   } catch (...) {
@@ -224,6 +241,8 @@ int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_
   }
   try {
     if (overlaps(l)) return ILQR_ERR_OVERLAP;
+    if (total == nullptr && is_small(l))
+      return small_impl(l, s.max_type != 0, &s, ilqr::GradNormOut{norm, nullptr, nullptr}, stream);
     return n_tensors <= ilqr::GRAD_CAP_SHORT ? clip_impl<ilqr::GRAD_CAP_SHORT>(l, s, total, norm, slots, stream)
                                              : clip_impl<ilqr::GRAD_CAP_LONG>(l, s, total, norm, slots, stream);
   } catch (...) {
