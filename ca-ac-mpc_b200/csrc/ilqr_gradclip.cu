@@ -237,6 +237,46 @@ __device__ __forceinline__ Vec<VB> load_vec(const char* p) {
   return *reinterpret_cast<const Vec<VB>*>(p);
 }
 
+// What L2 does with a line: a long list's two passes read it from L2 where they
+// can, and what will not be read again leaves it first.
+enum class Keep { USUAL, POLICY };
+
+__device__ __forceinline__ uint64_t policy_first_out() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
+__device__ __forceinline__ uint64_t policy_usual() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
+template <Keep K>
+__device__ __forceinline__ Vec<16> load_16(const char* p, uint64_t policy) {
+  if constexpr (K == Keep::USUAL) {
+    return load_vec<16>(p);
+  } else {
+    Vec<16> v;
+    asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=r"(v.w.x), "=r"(v.w.y), "=r"(v.w.z), "=r"(v.w.w)
+                 : "l"(p), "l"(policy)
+                 : "memory");
+    return v;
+  }
+}
+
+template <Keep K>
+__device__ __forceinline__ void store_16(char* p, const Vec<16>& v, uint64_t policy) {
+  if constexpr (K == Keep::USUAL)
+    *reinterpret_cast<Vec<16>*>(p) = v;
+  else
+    asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(p), "r"(v.w.x), "r"(v.w.y),
+                 "r"(v.w.z), "r"(v.w.w), "l"(policy)
+                 : "memory");
+}
+
 template <int DT, int VB>
 __device__ __forceinline__ void unpack_vec(const Vec<VB>& v, float* x) {
   if constexpr (VB == 2) {
@@ -294,8 +334,8 @@ __device__ __forceinline__ int head_of(const char* p, int64_t n) {
   return n < h ? (int)n : h;
 }
 
-template <int DT, bool MAX, int THREADS>
-__device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n) {
+template <int DT, bool MAX, Keep K>
+__device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n, uint64_t policy) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
   const int tid = threadIdx.x;
   const int h = head_of<DT>(p, n);
@@ -306,10 +346,10 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
   }
   p += h * SZ + tid * 16;
   int64_t left = (n - h) / VE - tid;  // vectors from this thread's first on
-  for (; left > (UN - 1) * THREADS; left -= UN * THREADS, p += UN * THREADS * 16) {
+  for (; left > (UN - 1) * BLK; left -= UN * BLK, p += UN * BLK * 16) {
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * THREADS * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_16<K>(p + u * BLK * 16, policy);
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
   if (left > 0) {
@@ -317,15 +357,15 @@ __device__ __forceinline__ void range_sum(Acc<MAX>& a, const char* p, int64_t n)
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       v[u].w = make_uint4(0, 0, 0, 0);
-      if (left > u * THREADS) v[u] = load_vec<16>(p + u * THREADS * 16);
+      if (left > u * BLK) v[u] = load_16<K>(p + u * BLK * 16, policy);
     }
     add_vecs<DT, 16, UN, MAX>(a, v);
   }
 }
 
 // out = c in; `in` may be `out`
-template <int DT, int THREADS>
-__device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c) {
+template <int DT, Keep K, int UN>
+__device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, const Coef& c, uint64_t policy) {
   constexpr int SZ = Type<DT>::SIZE, VE = 16 / SZ;
   const int tid = threadIdx.x;
   const int h = head_of<DT>(p, n);
@@ -335,7 +375,7 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     store_one<DT>(q + at, scaled<false>(load_one<DT>(p + at), c));
   }
   // from the end: what the sums read last is still in L2
-  const int64_t nv = (n - h) / VE, full = nv / (UN * THREADS) * (UN * THREADS);
+  const int64_t nv = (n - h) / VE, full = nv / (UN * BLK) * (UN * BLK);
   int64_t left = nv - full - tid;
   p += h * SZ + (full + tid) * 16;
   q += h * SZ + (full + tid) * 16;
@@ -343,19 +383,19 @@ __device__ __forceinline__ void range_scale(const char* p, char* q, int64_t n, c
     Vec<16> v[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * THREADS) v[u] = load_vec<16>(p + u * THREADS * 16);
+      if (left > u * BLK) v[u] = load_16<K>(p + u * BLK * 16, policy);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (left > u * THREADS) *reinterpret_cast<Vec<16>*>(q + u * THREADS * 16) = scale_vec<DT, 16, false>(v[u], c);
+      if (left > u * BLK) store_16<K>(q + u * BLK * 16, scale_vec<DT, 16, false>(v[u], c), policy);
   }
-  for (left = full; left > 0; left -= UN * THREADS) {
-    p -= UN * THREADS * 16;
-    q -= UN * THREADS * 16;
+  for (left = full; left > 0; left -= UN * BLK) {
+    p -= UN * BLK * 16;
+    q -= UN * BLK * 16;
     Vec<16> v[UN];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) v[u] = load_vec<16>(p + u * THREADS * 16);
+    for (int u = 0; u < UN; ++u) v[u] = load_16<K>(p + u * BLK * 16, policy);
 #pragma unroll
-    for (int u = 0; u < UN; ++u) *reinterpret_cast<Vec<16>*>(q + u * THREADS * 16) = scale_vec<DT, 16, false>(v[u], c);
+    for (int u = 0; u < UN; ++u) store_16<K>(q + u * BLK * 16, scale_vec<DT, 16, false>(v[u], c), policy);
   }
 }
 
@@ -392,21 +432,21 @@ __device__ __forceinline__ void span(const GradTable<CAP>& tab, int t, uint32_t 
   *n = (b < e.numel ? b : e.numel) - a;
 }
 
-template <bool MAX, int THREADS>
-__device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const void* in, int64_t at, int64_t n) {
+template <bool MAX, Keep K>
+__device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const void* in, int64_t at, int64_t n,
+                                          uint64_t policy) {
   const char* p = static_cast<const char*>(in);
-  if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX, THREADS>(a, p + at * 4, n);
-  else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX, THREADS>(a, p + at * 2, n);
-  else range_sum<ILQR_DTYPE_F16, MAX, THREADS>(a, p + at * 2, n);
+  if (dtype == ILQR_DTYPE_F32) range_sum<ILQR_DTYPE_F32, MAX, K>(a, p + at * 4, n, policy);
+  else if (dtype == ILQR_DTYPE_BF16) range_sum<ILQR_DTYPE_BF16, MAX, K>(a, p + at * 2, n, policy);
+  else range_sum<ILQR_DTYPE_F16, MAX, K>(a, p + at * 2, n, policy);
 }
 
 // Value by value: for coefficients below the floats' range, and for `in` and
 // `out` that lie differently in their 16-byte words.
-template <int THREADS>
 __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p, char* q, int64_t n, const Coef& c) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
 #pragma unroll 1
-  for (int64_t i = threadIdx.x; i < n; i += THREADS) {
+  for (int64_t i = threadIdx.x; i < n; i += BLK) {
     const char* from = p + i * sz;
     float x = dtype == ILQR_DTYPE_F32    ? load_one<ILQR_DTYPE_F32>(from)
               : dtype == ILQR_DTYPE_BF16 ? load_one<ILQR_DTYPE_BF16>(from)
@@ -419,47 +459,81 @@ __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p,
   }
 }
 
-template <int THREADS>
+template <Keep K, int UN>
 __device__ __forceinline__ void entry_scale(uint32_t dtype, const void* in, void* out, int64_t at, int64_t n,
-                                            const Coef& c) {
+                                            const Coef& c, uint64_t policy) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
   const char* p = static_cast<const char*>(in) + at * sz;
   char* q = static_cast<char*>(out) + at * sz;
   if (c.wide || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u))
-    entry_scale_apart<THREADS>(dtype, p, q, n, c);
-  else if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32, THREADS>(p, q, n, c);
-  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16, THREADS>(p, q, n, c);
-  else range_scale<ILQR_DTYPE_F16, THREADS>(p, q, n, c);
+    entry_scale_apart(dtype, p, q, n, c);
+  else if (dtype == ILQR_DTYPE_F32) range_scale<ILQR_DTYPE_F32, K, UN>(p, q, n, c, policy);
+  else if (dtype == ILQR_DTYPE_BF16) range_scale<ILQR_DTYPE_BF16, K, UN>(p, q, n, c, policy);
+  else range_scale<ILQR_DTYPE_F16, K, UN>(p, q, n, c, policy);
 }
 
-// Partial sums. Each block takes a contiguous run of chunks; with PER one sum
-// for each tensor in it, at slot block + tensor: slots of neighbours are
-// neighbours, and where a block ends with its tensor the one slot that falls
-// out is set to 0, the identity of both joins.
-template <int CAP, bool MAX, bool PER>
+// Chunks [k, end) of the list into a sum, t the tensor of chunk k.
+template <int CAP, bool MAX, Keep K>
+__device__ __forceinline__ void chunks_sum(Acc<MAX>& a, const GradTable<CAP>& tab, uint32_t k, uint32_t end, int t,
+                                           uint64_t policy) {
+  for (; k < end; ++t) {
+    const uint32_t stop = t + 1 < tab.n ? min(end, tab.e[t + 1].chunk0) : end;
+    int64_t at, n;
+    span(tab, t, k, stop, &at, &n);
+    entry_sum<MAX, K>(a, tab.e[t].dtype, tab.e[t].in, at, n, policy);
+    k = stop;
+  }
+}
+
+// Partial sums, one for each block, of equal contiguous runs of chunks.
+template <int CAP, bool MAX>
 __global__ void __launch_bounds__(BLK) grad_sum_kernel(const __grid_constant__ GradTable<CAP> tab, double* slots) {
+  __shared__ double sh[32];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
+  Acc<MAX> a;
+  chunks_sum<CAP, MAX, Keep::USUAL>(a, tab, k, first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x), find(tab, k), 0);
+  const double v = block_join<MAX>(value(a), sh);
+  if (threadIdx.x == 0) slots[blockIdx.x] = v;
+}
+
+// The same before the scaling of a long list: the blocks go through it together,
+// four chunks each at a time, so that its last part is read last; what lies
+// before the last keep_chunks leaves L2 first (300 MB, both passes, in runs and
+// so: 143 | 140 us; the sums alone are 47 | 49 us).
+template <int CAP, bool MAX>
+__global__ void __launch_bounds__(BLK) grad_sum_long_kernel(const __grid_constant__ GradTable<CAP> tab,
+                                                            uint32_t keep_chunks, double* slots) {
+  __shared__ double sh[32];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const uint64_t first = policy_first_out(), usual = policy_usual();
+  Acc<MAX> a;
+  for (uint32_t k = blockIdx.x * 4; k < tab.chunks; k += gridDim.x * 4)
+    chunks_sum<CAP, MAX, Keep::POLICY>(a, tab, k, min(k + 4, tab.chunks), find(tab, k),
+                                       tab.chunks - k > keep_chunks ? first : usual);
+  const double v = block_join<MAX>(value(a), sh);
+  if (threadIdx.x == 0) slots[blockIdx.x] = v;
+}
+
+// Partial sums for each tensor. Each block takes a contiguous run of chunks and
+// leaves one sum for each tensor in it at slot block + tensor: slots of
+// neighbours are neighbours, and where a block ends with its tensor the one slot
+// that falls out is set to 0, the identity of both joins.
+template <int CAP, bool MAX>
+__global__ void __launch_bounds__(BLK) grad_each_kernel(const __grid_constant__ GradTable<CAP> tab, double* slots) {
   __shared__ double sh[32];
   asm volatile("griddepcontrol.launch_dependents;");
   uint32_t k = first_chunk(blockIdx.x, tab.chunks, gridDim.x);
   const uint32_t k1 = first_chunk(blockIdx.x + 1, tab.chunks, gridDim.x);
   int t = find(tab, k);
-  if (PER && blockIdx.x > 0 && k == tab.e[t].chunk0 && threadIdx.x == 0) slots[blockIdx.x + t - 1] = 0.0;
-  Acc<MAX> a;
+  if (blockIdx.x > 0 && k == tab.e[t].chunk0 && threadIdx.x == 0) slots[blockIdx.x + t - 1] = 0.0;
   for (; k < k1; ++t) {
     const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
-    int64_t at, n;
-    span(tab, t, k, end, &at, &n);
-    entry_sum<MAX, BLK>(a, tab.e[t].dtype, tab.e[t].in, at, n);
-    if (PER) {
-      const double v = block_join<MAX>(value(a), sh);
-      if (threadIdx.x == 0) slots[blockIdx.x + t] = v;
-      a = Acc<MAX>();
-    }
-    k = end;
-  }
-  if (!PER) {
+    Acc<MAX> a;
+    chunks_sum<CAP, MAX, Keep::USUAL>(a, tab, k, end, t, 0);
     const double v = block_join<MAX>(value(a), sh);
-    if (threadIdx.x == 0) slots[blockIdx.x] = v;
+    if (threadIdx.x == 0) slots[blockIdx.x + t] = v;
+    k = end;
   }
 }
 
@@ -496,23 +570,27 @@ __global__ void __launch_bounds__(BLK) grad_join_kernel(const __grid_constant__ 
   if ((threadIdx.x & 31) == 0) out.tensor_norms[t] = (float)norm_of(v, MAX);
 }
 
-// out = c in over chunks [k0, k1), from the end. In place a coefficient of 1
-// leaves the values where they are.
-template <int CAP, int THREADS>
-__device__ __forceinline__ void chunks_scale(const GradTable<CAP>& tab, uint32_t k0, uint32_t k1, int t, const Coef& c) {
+// out = c in over chunks [k0, k1), from the end (what the sums read last is still
+// in L2), t the tensor of chunk k1 - 1. In place a coefficient of 1 leaves the
+// values where they are.
+template <int CAP, Keep K, int UN>
+__device__ __forceinline__ void chunks_scale(const GradTable<CAP>& tab, uint32_t k0, uint32_t k1, int t, const Coef& c,
+                                             uint64_t policy) {
+  if (c.d == 1.0 && tab.in_place) return;
   for (; k1 > k0; --t) {
     const GradEntry& e = tab.e[t];
     const uint32_t begin = max(k0, e.chunk0);
     if (!(c.d == 1.0 && e.in == e.out)) {
       int64_t at, n;
       span(tab, t, begin, k1, &at, &n);
-      entry_scale<THREADS>(e.dtype, e.in, e.out, at, n, c);
+      entry_scale<K, UN>(e.dtype, e.in, e.out, at, n, c, policy);
     }
     k1 = begin;
   }
 }
 
-// Every block joins the partial sums for itself, in the same order.
+// A wave of blocks with a run of chunks each; every block joins the partial sums
+// for itself, in the same order.
 template <int CAP>
 __global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
                                                             const double* slots, int64_t n_slots, float* norm) {
@@ -524,7 +602,24 @@ __global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constan
   const double total = s.max_type ? join_slots<true>(slots, n_slots, sh) : join_slots<false>(slots, n_slots, sh);
   const double nrm = norm_of(total, s.max_type);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
-  chunks_scale<CAP, BLK>(tab, k0, k1, t, coef_of(nrm, s.max_norm, s.eps));
+  chunks_scale<CAP, Keep::USUAL, UN>(tab, k0, k1, t, coef_of(nrm, s.max_norm, s.eps), 0);
+}
+
+// A long list: the blocks go through it together from the end, GRAD_LONG_STEP
+// chunks at a time. The total is one value.
+template <int CAP>
+__global__ void __launch_bounds__(BLK, 8) grad_scale_long_kernel(const __grid_constant__ GradTable<CAP> tab,
+                                                                 GradScale s, const double* total, float* norm) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double nrm = norm_of(*total, s.max_type);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
+  const Coef c = coef_of(nrm, s.max_norm, s.eps);
+  if (c.d == 1.0 && tab.in_place) return;
+  const uint64_t policy = policy_first_out();
+  for (uint32_t past = blockIdx.x * GRAD_LONG_STEP; past < tab.chunks; past += gridDim.x * GRAD_LONG_STEP) {
+    const uint32_t k1 = tab.chunks - past, k0 = k1 > GRAD_LONG_STEP ? k1 - GRAD_LONG_STEP : 0;
+    chunks_scale<CAP, Keep::POLICY, 2>(tab, k0, k1, find(tab, k1 - 1), c, policy);
+  }
 }
 
 // A short list by one cluster, in one launch and without a workspace: the
@@ -536,22 +631,17 @@ __global__ void __launch_bounds__(BLK) grad_small_kernel(const __grid_constant__
   const uint32_t rank = cluster_rank(), n_blocks = cluster_size();
   const uint32_t k0 = first_chunk(rank, tab.chunks, n_blocks), k1 = first_chunk(rank + 1, tab.chunks, n_blocks);
   Acc<MAX> a;
-  int t = 0;
-  if (k0 < k1) t = find(tab, k0);
-  for (uint32_t k = k0; k < k1; ++t) {
-    const uint32_t end = t + 1 < tab.n ? min(k1, tab.e[t + 1].chunk0) : k1;
-    int64_t at, n;
-    span(tab, t, k, end, &at, &n);
-    entry_sum<MAX, BLK>(a, tab.e[t].dtype, tab.e[t].in, at, n);
-    k = end;
-  }
+  if (k0 < k1) chunks_sum<CAP, MAX, Keep::USUAL>(a, tab, k0, k1, find(tab, k0), 0);
   const double total = cluster_join<MAX>(block_join<MAX>(value(a), sh), sh + 32);
   const double nrm = norm_of(total, MAX);
   if (rank == 0 && threadIdx.x == 0) {
     if (out.norm != nullptr) *out.norm = (float)nrm;
     if (out.total != nullptr) *out.total = total;
   }
-  if constexpr (SCALE) chunks_scale<CAP, BLK>(tab, k0, k1, t - 1, coef_of(nrm, s.max_norm, s.eps));
+  if constexpr (SCALE) {
+    if (k0 < k1)
+      chunks_scale<CAP, Keep::USUAL, UN>(tab, k0, k1, find(tab, k1 - 1), coef_of(nrm, s.max_norm, s.eps), 0);
+  }
   cluster_wait();
 }
 
@@ -993,13 +1083,19 @@ cudaError_t launch(void (*kernel)(K...), unsigned grid, bool dependent, cudaStre
 }  // namespace
 
 template <int CAP>
-cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, bool per_tensor, double* slots,
+cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, uint32_t keep_chunks, double* slots,
                             cudaStream_t stream) {
-  if (max_type)
-    return per_tensor ? launch(grad_sum_kernel<CAP, true, true>, grid, false, stream, tab, slots)
-                      : launch(grad_sum_kernel<CAP, true, false>, grid, false, stream, tab, slots);
-  return per_tensor ? launch(grad_sum_kernel<CAP, false, true>, grid, false, stream, tab, slots)
-                    : launch(grad_sum_kernel<CAP, false, false>, grid, false, stream, tab, slots);
+  if (keep_chunks > 0)
+    return max_type ? launch(grad_sum_long_kernel<CAP, true>, grid, false, stream, tab, keep_chunks, slots)
+                    : launch(grad_sum_long_kernel<CAP, false>, grid, false, stream, tab, keep_chunks, slots);
+  return max_type ? launch(grad_sum_kernel<CAP, true>, grid, false, stream, tab, slots)
+                  : launch(grad_sum_kernel<CAP, false>, grid, false, stream, tab, slots);
+}
+
+template <int CAP>
+cudaError_t launch_grad_each(const GradTable<CAP>& tab, int grid, bool max_type, double* slots, cudaStream_t stream) {
+  return max_type ? launch(grad_each_kernel<CAP, true>, grid, false, stream, tab, slots)
+                  : launch(grad_each_kernel<CAP, false>, grid, false, stream, tab, slots);
 }
 
 template <int CAP>
@@ -1019,6 +1115,13 @@ template <int CAP>
 cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
                               int64_t n_slots, float* norm, bool dependent, cudaStream_t stream) {
   return launch(grad_scale_kernel<CAP>, grid, dependent, stream, tab, s, slots, n_slots, norm);
+}
+
+template <int CAP>
+cudaError_t launch_grad_scale_long(const GradTable<CAP>& tab, const GradScale& s, const double* total, float* norm,
+                                   bool dependent, cudaStream_t stream) {
+  const unsigned grid = min((tab.chunks + GRAD_LONG_STEP - 1) / GRAD_LONG_STEP, GRAD_LONG_GRID);
+  return launch(grad_scale_long_kernel<CAP>, grid, dependent, stream, tab, s, total, norm);
 }
 
 template <int CAP, bool MAX, bool SCALE>
@@ -1050,11 +1153,14 @@ cudaError_t launch_grad_small(const GradTable<CAP>& tab, bool max_type, const Gr
 }
 
 #define INSTANTIATE(CAP)                                                                                              \
-  template cudaError_t launch_grad_sum<CAP>(const GradTable<CAP>&, int, bool, bool, double*, cudaStream_t);           \
+  template cudaError_t launch_grad_sum<CAP>(const GradTable<CAP>&, int, bool, uint32_t, double*, cudaStream_t);       \
+  template cudaError_t launch_grad_each<CAP>(const GradTable<CAP>&, int, bool, double*, cudaStream_t);                \
   template cudaError_t launch_grad_join<CAP>(const GradTable<CAP>*, int, const double*, bool, const double*, int64_t, \
                                              const GradNormOut&, bool, cudaStream_t);                                 \
   template cudaError_t launch_grad_scale<CAP>(const GradTable<CAP>&, int, const GradScale&, const double*, int64_t,   \
-                                              float*, bool, cudaStream_t);
+                                              float*, bool, cudaStream_t);                                            \
+  template cudaError_t launch_grad_scale_long<CAP>(const GradTable<CAP>&, const GradScale&, const double*, float*,    \
+                                                   bool, cudaStream_t);
 template cudaError_t launch_grad_small<GRAD_CAP_SHORT>(const GradTable<GRAD_CAP_SHORT>&, bool, const GradScale*,
                                                        const GradNormOut&, cudaStream_t);
 INSTANTIATE(GRAD_CAP_SHORT)

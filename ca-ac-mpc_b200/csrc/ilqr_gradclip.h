@@ -30,14 +30,25 @@ struct GradTable {
   int32_t n;
   uint32_t chunks;
   uint32_t chunk_bytes;
-  uint32_t pad;
+  uint32_t in_place;  // whether every out is its in
   GradEntry e[CAP];
 };
 
-// Partial sums of a launch: one per block, or with per-tensor sums one per
-// (block, tensor) that meet, at slot block + tensor.
+// A wave: four blocks of 256 threads on each SM.
 constexpr int GRAD_MAX_GRID = 148 * 4;
 constexpr uint32_t GRAD_CHUNK_BYTES = 16384;
+
+// A list beyond this size does not stay in L2 between the two passes (300 MB,
+// us as a shorter list | as a long one: 155 | 140; 80 MB 42 | 40, 48 MB 26 | 27).
+// Its first pass leaves the last GRAD_KEEP_BYTES for the second to find; its
+// scaling takes GRAD_LONG_STEP chunks a block at a time, GRAD_LONG_GRID blocks at
+// most: with fewer of them, each with a larger share, the last to end is waited
+// for (a wave of eight on an SM: 137 us for 275 MB, two 135, three 131, four 129,
+// one for every step 129).
+constexpr int64_t GRAD_LONG_BYTES = 64 << 20;
+constexpr int64_t GRAD_KEEP_BYTES = 90 << 20;
+constexpr uint32_t GRAD_LONG_STEP = 2;
+constexpr unsigned GRAD_LONG_GRID = 148 * 8 * 4;
 
 // A list up to this size is short: one cluster takes it, in one launch instead
 // of two (two | one, us of GPU time and of an eager call: clipping 128 KB
@@ -99,9 +110,14 @@ constexpr uint32_t GRAD_MAX_STAGED = 224 * 1024;
 // Segments from this many bytes on move by bulk copies.
 constexpr uint32_t GRAD_MIN_BULK = 256;
 
+// Partial sums of a launch: one for each block. keep_chunks > 0: what lies before
+// that many of the last chunks will not be found in L2 and leaves it first.
 template <int CAP>
-cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, bool per_tensor, double* slots,
+cudaError_t launch_grad_sum(const GradTable<CAP>& tab, int grid, bool max_type, uint32_t keep_chunks, double* slots,
                             cudaStream_t stream);
+// One for each (block, tensor) that meet, at slot block + tensor.
+template <int CAP>
+cudaError_t launch_grad_each(const GradTable<CAP>& tab, int grid, bool max_type, double* slots, cudaStream_t stream);
 // Joins n_slots partials into the norm; with tab != nullptr also the norms of
 // its tensors from the launch's own slots (tab_slots, grid).
 template <int CAP>
@@ -111,6 +127,9 @@ cudaError_t launch_grad_join(const GradTable<CAP>* tab, int grid, const double* 
 template <int CAP>
 cudaError_t launch_grad_scale(const GradTable<CAP>& tab, int grid, const GradScale& s, const double* slots,
                               int64_t n_slots, float* norm, bool dependent, cudaStream_t stream);
+template <int CAP>
+cudaError_t launch_grad_scale_long(const GradTable<CAP>& tab, const GradScale& s, const double* total, float* norm,
+                                   bool dependent, cudaStream_t stream);
 // A short list in one launch; s == nullptr: its norm only.
 template <int CAP>
 cudaError_t launch_grad_small(const GradTable<CAP>& tab, bool max_type, const GradScale* s, const GradNormOut& out,

@@ -83,25 +83,27 @@ uint64_t chunks_of(int64_t numel, int32_t dtype, uint32_t chunk_bytes) {
   return c > 0 ? c : 1;
 }
 
-// Whether a list is short enough for the one-launch form.
-bool is_small(const List& l) {
-  if (l.n > ilqr::GRAD_CAP_SHORT) return false;
+int64_t bytes_of(const List& l) {
   int64_t bytes = 0;
   for (int32_t i = 0; i < l.n; ++i) bytes += l.numel[i] * size_of(l.dtype[i]);
-  return bytes <= ilqr::GRAD_SMALL_BYTES;
+  return bytes;
 }
+
+// Whether a list is short enough for the one-launch form.
+bool is_small(const List& l) { return l.n <= ilqr::GRAD_CAP_SHORT && bytes_of(l) <= ilqr::GRAD_SMALL_BYTES; }
 
 template <int CAP>
 void fill(GradTable<CAP>& tab, const List& l, int32_t first, int32_t n,
           uint32_t chunk_bytes = ilqr::GRAD_CHUNK_BYTES) {
   tab.n = n;
   tab.chunk_bytes = chunk_bytes;
-  tab.pad = 0;
+  tab.in_place = 1;
   uint64_t at = 0;
   for (int32_t i = 0; i < n; ++i) {
     const int32_t k = first + i;
     tab.e[i] = GradEntry{l.in[k], l.out != nullptr ? l.out[k] : nullptr, l.numel[k], (uint32_t)at,
                          (uint32_t)l.dtype[k]};
+    if (tab.e[i].in != tab.e[i].out) tab.in_place = 0;
     at += chunks_of(l.numel[k], l.dtype[k], chunk_bytes);
   }
   tab.chunks = (uint32_t)at;
@@ -126,7 +128,8 @@ int norm_impl(const List& l, bool max_type, const ilqr::GradNormOut& o, double* 
     const int32_t n = std::min<int32_t>(CAP, l.n - first);
     fill(*tab, l, first, n);
     const int grid = grid_of(tab->chunks);
-    cudaError_t e = ilqr::launch_grad_sum(*tab, grid, max_type, per, slots + used, stream);
+    cudaError_t e = per ? ilqr::launch_grad_each(*tab, grid, max_type, slots + used, stream)
+                        : ilqr::launch_grad_sum(*tab, grid, max_type, 0u, slots + used, stream);
     if (e != cudaSuccess) return ILQR_ERR_CUDA;
     const double* mine = slots + used;
     used += grid + (per ? n - 1 : 0);
@@ -145,6 +148,9 @@ template <int CAP>
 int clip_impl(const List& l, const ilqr::GradScale& s, const double* total, float* norm, double* slots,
               cudaStream_t stream) {
   const std::unique_ptr<GradTable<CAP>> tab(new GradTable<CAP>);
+  const bool is_long = bytes_of(l) > ilqr::GRAD_LONG_BYTES;
+  const uint32_t keep = is_long ? (uint32_t)(ilqr::GRAD_KEEP_BYTES / ilqr::GRAD_CHUNK_BYTES) : 0;
+  const bool mx = s.max_type != 0;
   const double* from = total;
   int64_t used = 1;
   if (total == nullptr) {
@@ -152,25 +158,26 @@ int clip_impl(const List& l, const ilqr::GradScale& s, const double* total, floa
     for (int32_t first = 0; first < l.n; first += CAP) {
       fill(*tab, l, first, std::min<int32_t>(CAP, l.n - first));
       const int grid = grid_of(tab->chunks);
-      if (ilqr::launch_grad_sum(*tab, grid, s.max_type != 0, false, slots + used, stream) != cudaSuccess)
-        return ILQR_ERR_CUDA;
+      if (ilqr::launch_grad_sum(*tab, grid, mx, keep, slots + used, stream) != cudaSuccess) return ILQR_ERR_CUDA;
       used += grid;
     }
     from = slots;
-    if (used > MANY_SLOTS) {
+    if (is_long || used > MANY_SLOTS) {
       const ilqr::GradNormOut o{nullptr, nullptr, slots + used};
-      if (ilqr::launch_grad_join<CAP>(nullptr, 0, nullptr, s.max_type != 0, slots, used, o, true, stream) !=
-          cudaSuccess)
+      if (ilqr::launch_grad_join<CAP>(nullptr, 0, nullptr, mx, slots, used, o, true, stream) != cudaSuccess)
         return ILQR_ERR_CUDA;
       from = slots + used;
       used = 1;
     }
   }
+  const bool dependent = total == nullptr;
   for (int32_t first = 0; first < l.n; first += CAP) {
     if (l.n > CAP || total != nullptr) fill(*tab, l, first, std::min<int32_t>(CAP, l.n - first));
-    if (ilqr::launch_grad_scale(*tab, grid_of(tab->chunks), s, from, used, first == 0 ? norm : nullptr,
-                                total == nullptr, stream) != cudaSuccess)
-      return ILQR_ERR_CUDA;
+    float* out = first == 0 ? norm : nullptr;
+    const cudaError_t e =
+        is_long ? ilqr::launch_grad_scale_long(*tab, s, from, out, dependent, stream)
+                : ilqr::launch_grad_scale(*tab, grid_of(tab->chunks), s, from, used, out, dependent, stream);
+    if (e != cudaSuccess) return ILQR_ERR_CUDA;
   }
   return ILQR_OK;
 }
