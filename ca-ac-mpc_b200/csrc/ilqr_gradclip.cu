@@ -800,6 +800,30 @@ __device__ __forceinline__ void staged_scale(uint32_t dtype, char* p, uint32_t n
   else staged_scale<ILQR_DTYPE_F16>(p, n, c, lane, step);
 }
 
+// Zeros in their place, or scaled by a coefficient below the floats' range.
+__device__ __noinline__ void staged_apart(uint32_t dtype, char* p, uint32_t n, const Coef& c, bool zero, uint32_t lane,
+                                          uint32_t step) {
+  if (zero) {
+#pragma unroll 1
+    for (uint32_t i = lane; i < n; i += step) *reinterpret_cast<Vec<16>*>(p + i * 16) = Vec<16>{};
+  } else if (dtype == ILQR_DTYPE_F32) {
+#pragma unroll 1
+    for (uint32_t i = lane; i < n * 4; i += step) {
+      float* x = reinterpret_cast<float*>(p) + i;
+      *x = scaled<true>(*x, c);
+    }
+  } else {
+#pragma unroll 1
+    for (uint32_t i = lane; i < n * 8; i += step) {
+      char* at = p + i * 2;
+      if (dtype == ILQR_DTYPE_BF16)
+        store_one<ILQR_DTYPE_BF16>(at, scaled<true>(load_one<ILQR_DTYPE_BF16>(at), c));
+      else
+        store_one<ILQR_DTYPE_F16>(at, scaled<true>(load_one<ILQR_DTYPE_F16>(at), c));
+    }
+  }
+}
+
 // The same from global memory, for slices that shared memory cannot hold.
 template <int DT, int VB>
 __device__ __forceinline__ void row_sum(Acc<false>& a, const RowTensor& r, int64_t b, uint32_t lane, uint32_t step) {
@@ -923,7 +947,7 @@ __device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, 
 // memory is read once and written once. CLUSTER: the blocks of a cluster share
 // one element.
 template <int G, int THREADS, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constant__ RowTable tab) {
+__global__ void __launch_bounds__(THREADS, G <= 32 ? 10 : 1) grad_rows_kernel(const __grid_constant__ RowTable tab) {
   extern __shared__ __align__(16) char staged[];
   __shared__ double sh[33];
   __shared__ uint64_t bars[THREADS / G];
@@ -997,13 +1021,12 @@ __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constan
   if (lane == 0 && tab.norms != nullptr && (!CLUSTER || cluster_rank() == 0)) tab.norms[b] = (float)nrm;
   const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
   const bool zero = tab.zero_nonfinite && !isfinite(nrm);
-  if (zero || c.wide) {
-    for (int k = 0; k < tab.n; ++k) row_apart(tensors[k], b, c, zero, lane, G);
-    if constexpr (CLUSTER) cluster_wait();
-    return;
-  }
-  if (c.d != 1.0) {
-    if (tab.one_dtype) {
+  const bool changed = c.d != 1.0 || zero;
+  if (changed) {
+    if (zero || c.wide) {
+      for (int k = 0; k < tab.n; ++k)
+        staged_apart(tensors[k].dtype, mine + tensors[k].staged, tensors[k].staged_vecs, c, zero, lane, G);
+    } else if (tab.one_dtype) {
       staged_scale(tab.t[0].dtype, mine, staged_bytes / 16, c, lane, G);
     } else {
       for (int k = 0; k < tab.n; ++k)
@@ -1015,13 +1038,13 @@ __global__ void __launch_bounds__(THREADS) grad_rows_kernel(const __grid_constan
   if (tab.bulk && lane < LANES) {
     for (int k = 0; k < tab.n; ++k) {
       const RowTensor& r = tensors[k];
-      if (r.bulk && !(c.d == 1.0 && r.in == r.out)) bulk_out(r, b, to + r.staged, lane, LANES);
+      if (r.bulk && (changed || r.in != r.out)) bulk_out(r, b, to + r.staged, lane, LANES);
     }
     bulk_commit();
   }
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tensors[k];
-    if (c.d == 1.0 && r.in == r.out) continue;
+    if (!changed && r.in == r.out) continue;
     if (r.bulk) {
       if (r.bulk == ROW_BULK_ENDS) ends<true>(r, b, mine + r.staged, lane, G);
       continue;
