@@ -116,8 +116,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     """Clip the gradients of the policy's parameters in place by their norm
     together, as the update does between its backward and the optimiser's step
     (th.nn.utils.clip_grad_norm_(policy.parameters(), max_grad_norm),
-    stable_baselines3/ppo/ppo.py:274-277): the same arguments and result, the
-    norm before clipping as a device scalar. Parameters without a gradient are
+    stable_baselines3/ppo/ppo.py:274-277): its arguments (but foreach) and its
+    result, the norm before clipping as a device scalar. Parameters without a gradient are
     passed over; parameters on several devices are clipped by their joint
     norm. norm_type: 2 or inf. Nothing reads back to the host unless
     error_if_nonfinite asks for it."""

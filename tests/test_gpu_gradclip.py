@@ -488,3 +488,151 @@ def test_two_graphs_replayed_with_new_values():
             assert all(torch.equal(a, b) for a, b in zip(want, out))
             wr, w0 = nat.clip_grad_elements(rows, 3.0)
             assert torch.equal(w0, rn) and torch.equal(wr[0], ro[0])
+
+
+# ---- what lies around, and the first call --------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [5, 56, 131, 700, 2900, 40_003])
+def test_elements_leave_what_lies_around_them(dtype, width):
+    """Slices at every offset within 16 bytes of a wider array, in place and into
+    another array at the same and at another offset: nothing else is written."""
+    B, room = 6, 16
+    for at in range(0, 9, 1 if width < 200 else 3):
+        for d in (0, 1):
+            shape = (B, width + room) if d == 0 else (3, B, width + room)
+            base = torch.full(shape, 7.0, dtype=dtype, device=DEV)
+            x = base[..., at:at + width]
+            x.copy_(_values(tuple(x.shape), dtype, width + at))
+            start = base.clone()
+            other = torch.full_like(base, 5.0)
+            for to in (at, at + 1):
+                y = other[..., to:to + width]
+                want, n = _check_elements([x], [d], math.sqrt(width) * 0.9, out=[y])
+                kept = other.clone()
+                kept[..., to:to + width] = 5.0
+                assert torch.equal(kept, torch.full_like(kept, 5.0)) and torch.equal(base, start)
+                if to == at:  # the same words, so the same order of the sums
+                    done = y.clone()
+                other.fill_(5.0)
+            _check_elements([x], [d], math.sqrt(width) * 0.9, out=[x])
+            assert torch.equal(x, done)
+            start[..., at:at + width] = x
+            assert torch.equal(base, start)
+
+
+def test_elements_without_values():
+    for dims, x in (([0], [torch.zeros(4, 0, device=DEV)]), ([1], [torch.zeros(0, 4, 3, device=DEV)])):
+        got, n = nat.clip_grad_elements(x, 1.0, batch_dims=dims)
+        assert n.tolist() == [0.0] * 4 and got[0].shape == x[0].shape
+    got, n = nat.clip_grad_elements([torch.zeros(0, 9, device=DEV)], 1.0)
+    assert n.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_list_leaves_what_lies_around_it(dtype):
+    """Views at every offset, small and long lists, in place and into outputs
+    that lie otherwise in their 16-byte words."""
+    for n in (3, 100, 5000, 70_001):
+        for at in (0, 1, 3, 7):
+            base = torch.full((n + 20,), 7.0, dtype=dtype, device=DEV)
+            x = base[at:at + n]
+            x.copy_(_values((n,), dtype, n))
+            other = torch.full_like(base, 5.0)
+            m = 0.5 * _norm64([_wide(x)])
+            c = _coef64(_norm64([_wide(x)]), m)
+            want = _wide(x) * c
+            for to in (at, at + 1, at + 4):
+                y = other[to:to + n]
+                nat.clip_grad_norm([x], m, out=[y])
+                _close_values(y, want)
+                y.fill_(5.0)
+                assert torch.equal(other, torch.full_like(other, 5.0))
+            nat.clip_grad_norm([x], m, out=[x])
+            _close_values(x, want)
+            rest = torch.cat([base[:at], base[at + n:]])
+            assert torch.equal(rest, torch.full_like(rest, 7.0))
+
+
+@pytest.mark.parametrize("dtype,n", [(F32, 20_000_001), (BF16, 40_000_003)])
+def test_lists_beyond_l2(dtype, n):
+    """The form for lists that do not stay in L2, out of place, in place, below
+    the bound, and with a total from elsewhere."""
+    flat = _values((n,), dtype, 1)
+    sizes = [n // 3, 1, n // 2, 17]
+    sizes.append(n - sum(sizes))
+    x = list(flat.split(sizes))
+    before = _wide(flat)
+    norm = float(np.sqrt(np.square(before).sum()))
+    c = _coef64(norm, 0.3 * norm)
+    got, nn = nat.clip_grad_norm(x, 0.3 * norm)
+    _close_norm(nn, norm)
+    _close_values(torch.cat(got), before * c)
+    again, _ = nat.clip_grad_norm(x, 0.3 * norm, total=nat.grad_norm_total(x))
+    _close_values(torch.cat(again), before * c)
+    nat.clip_grad_norm(x, 2.0 * norm, out=x)
+    assert np.array_equal(_wide(flat), before)
+    top = float(np.abs(before).max())
+    got, nn = nat.clip_grad_norm(x, 0.5 * top, norm_type=math.inf)
+    assert float(nn) == np.float32(top)
+    _close_values(torch.cat(got), before * _coef64(top, 0.5 * top))
+    nat.clip_grad_norm(x, 0.3 * norm, out=x)
+    _close_values(flat, before * c)
+
+
+PROGRAM = """
+import sys
+sys.path[:0] = [{root!r}, {pkg!r}]
+import torch
+import ilqr_native as nat
+x = [torch.ones(100_000, device="cuda"), torch.ones(3, device="cuda")]
+y = [torch.ones(5, 700, device="cuda"), torch.ones(5, 40_000, device="cuda")]
+s = torch.cuda.Stream()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    a, n = nat.clip_grad_norm(x, 1.0)
+    b, m = nat.clip_grad_elements(y, 1.0)
+    k = nat.grad_norm(x, per_tensor=True)
+g.replay()
+torch.cuda.synchronize()
+assert abs(float(n) - 100_003 ** 0.5) < 1e-3 and abs(float(m[3]) - 40_700 ** 0.5) < 1e-3
+assert abs(float(a[0][5]) * float(n) - 1) < 1e-5 and abs(float(b[1][4, 9]) * float(m[4]) - 1) < 1e-5
+"""
+
+
+def test_first_calls_of_a_process_are_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", PROGRAM.format(root=root, pkg=os.path.join(root, "ca-ac-mpc_b200"))],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_two_threads_at_once():
+    """Calls from two Python threads on streams of their own."""
+    import threading
+    data = [[_values((60_000,), F32, k), _values((40, 3000), BF16, 9 + k)] for k in range(2)]
+    want = [(nat.clip_grad_norm(d, 2.0), nat.clip_grad_elements(d[1:], 2.0)) for d in data]
+    torch.cuda.synchronize()
+    fails = []
+
+    def work(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                (a, n), (b, m) = nat.clip_grad_norm(data[k], 2.0), nat.clip_grad_elements(data[k][1:], 2.0)
+                s.synchronize()
+                (a0, n0), (b0, m0) = want[k]
+                same = torch.equal(n, n0) and torch.equal(m, m0) and all(map(torch.equal, a + b, a0 + b0))
+                if not same:
+                    fails.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not fails
