@@ -947,7 +947,7 @@ __device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, 
 // memory is read once and written once. CLUSTER: the blocks of a cluster share
 // one element.
 template <int G, int THREADS, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, G <= 32 ? 10 : 1) grad_rows_kernel(const __grid_constant__ RowTable tab) {
+__global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1) grad_rows_kernel(const __grid_constant__ RowTable tab) {
   extern __shared__ __align__(16) char staged[];
   __shared__ double sh[33];
   __shared__ uint64_t bars[THREADS / G];
@@ -1001,7 +1001,7 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 10 : 1) grad_rows_kernel(co
     else threads_in<2>(r, b, to + r.staged, lane, G);
     // zeros after it, to a whole word
     const uint32_t end = r.n_seg * r.seg_bytes;
-    if (lane < (-end & 15u) / 2) *reinterpret_cast<uint16_t*>(mine + r.staged + end + 2 * lane) = 0;
+    for (uint32_t x = lane * 2; x < (-end & 15u); x += G * 2) *reinterpret_cast<uint16_t*>(mine + r.staged + end + x) = 0;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   group_sync<G>();  // the threads' copies and the barrier's set-up
@@ -1237,13 +1237,21 @@ cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned clust
 cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // Threads for an element by what it stages. More threads cost instructions
   // that every element repeats (its records, the join, square root and quotient),
-  // fewer leave the additions of long elements to few: us at 8 | 32 | 64 | 128
-  // threads, by bytes of an element (number of elements):
-  //   266 (100000)  19 | 58 | 122 | 212     8442 (16384)   82 | 49 | 52 | 72
-  //  1722 (40000)   26 | 41 |  78 | 128    16842 (16384)   -- | 87 | 87 | 86
-  //  2280 (16384)   23 | 18 |  26 |  41    24534 (4096)    -- | 64 | 53 | 49
-  //  5642 (16384)   38 | 31 |  33 |  46    42042 (65536)   -- | 1030 | 930 | 880
+  // fewer leave the additions of long elements to few: us by threads, bytes of an
+  // element and number of elements:
+  //     bytes (elements)    4     8    16    32    64   128
+  //       266 (100000)     15    19    32    55   122   212
+  //       602  (60000)     17    18    25    40    83   135
+  //      1722  (40000)     30    26    28    39    78   128
+  //      2282  (65536)           49    49    52
+  //      4242  (16384)           37    28    27    40    61
+  //      8442  (16384)           82    57    49    52    72
+  //     16842  (16384)                 112   87    87    86
+  //     24534   (4096)                  92   64    53    49
+  //     42042  (65536)                     1030   930   880
+  if (tab.staged_bytes <= 640) return launch_rows<4, 64>(tab, stream);
   if (tab.staged_bytes <= 2048) return launch_rows<8, 128>(tab, stream);
+  if (tab.staged_bytes <= 4096) return launch_rows<16, 128>(tab, stream);
   if (tab.staged_bytes <= 12288) return launch_rows<32, 128>(tab, stream);
   if (tab.staged_bytes <= 20480) return launch_rows<64, 64>(tab, stream);
   if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream);
