@@ -119,6 +119,12 @@ size_t slots_of(int32_t n) {
 
 constexpr int64_t MANY_SLOTS = 4096;  // beyond this the blocks of the scaling do not each join them
 
+// The join of partial sums alone (no tensors' norms, so no table of them).
+cudaError_t join_all(bool max_type, const double* slots, int64_t n_slots, const ilqr::GradNormOut& o,
+                     cudaStream_t stream) {
+  return ilqr::launch_grad_join<ilqr::GRAD_CAP_SHORT>(nullptr, 0, nullptr, max_type, slots, n_slots, o, true, stream);
+}
+
 template <int CAP>
 int norm_impl(const List& l, bool max_type, const ilqr::GradNormOut& o, double* slots, cudaStream_t stream) {
   const std::unique_ptr<GradTable<CAP>> tab(new GradTable<CAP>);
@@ -137,7 +143,8 @@ int norm_impl(const List& l, bool max_type, const ilqr::GradNormOut& o, double* 
     if (per || last) {
       ilqr::GradNormOut part = o;
       if (per) part.tensor_norms = o.tensor_norms + first;
-      e = ilqr::launch_grad_join<CAP>(per ? tab.get() : nullptr, grid, mine, max_type, slots, used, part, last, stream);
+      e = per ? ilqr::launch_grad_join(tab.get(), grid, mine, max_type, slots, used, part, last, stream)
+              : join_all(max_type, slots, used, part, stream);
       if (e != cudaSuccess) return ILQR_ERR_CUDA;
     }
   }
@@ -164,8 +171,7 @@ int clip_impl(const List& l, const ilqr::GradScale& s, const double* total, floa
     from = slots;
     if (is_long || used > MANY_SLOTS) {
       const ilqr::GradNormOut o{nullptr, nullptr, slots + used};
-      if (ilqr::launch_grad_join<CAP>(nullptr, 0, nullptr, mx, slots, used, o, true, stream) != cudaSuccess)
-        return ILQR_ERR_CUDA;
+      if (join_all(mx, slots, used, o, stream) != cudaSuccess) return ILQR_ERR_CUDA;
       from = slots + used;
       used = 1;
     }
@@ -243,8 +249,7 @@ int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_
     if (norm == nullptr) return ILQR_OK;
     if (total == nullptr) return status_of(cudaMemsetAsync(norm, 0, sizeof(float), stream));
     const ilqr::GradNormOut o{norm, nullptr, nullptr};
-    return status_of(ilqr::launch_grad_join<ilqr::GRAD_CAP_SHORT>(nullptr, 0, nullptr, s.max_type != 0, total, 1, o,
-                                                                  true, stream));
+    return status_of(join_all(s.max_type != 0, total, 1, o, stream));
   }
   try {
     if (overlaps(l)) return ILQR_ERR_OVERLAP;
