@@ -681,7 +681,7 @@ __device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
 }
 
 // How a slice gets to shared memory and back. Long segments move by bulk
-// copies, one each, issued by the lanes of one warp: each segment has a place of
+// copies, one each, issued by all threads: each segment has a place of
 // whole 16-byte words, lies there at its address modulo 16, and the copy takes
 // its whole words. What is left at its two ends moves value by value, and zeros
 // fill the place, so that sums and products run over whole words. Other slices
@@ -700,12 +700,13 @@ __device__ __forceinline__ Piece piece_of(const RowTensor& r, const char* p) {
   return c;
 }
 
-// Returns the bytes that this lane's copies bring.
-__device__ __forceinline__ uint32_t bulk_in(const RowTensor& r, int64_t b, uint32_t to, uint64_t* bar, uint32_t lane,
-                                            uint32_t lanes) {
+// Every `issuers`-th segment from the issuer's own; returns the bytes that these
+// copies bring.
+__device__ __forceinline__ uint32_t bulk_in(const RowTensor& r, int64_t b, uint32_t to, uint64_t* bar, uint32_t issuer,
+                                            uint32_t issuers) {
   const char* p = r.in + b * r.in_row;
   uint32_t bytes = 0;
-  for (uint32_t s = lane; s < r.n_seg; s += lanes) {
+  for (uint32_t s = issuer; s < r.n_seg; s += issuers) {
     const char* from = p + s * r.in_seg;
     const Piece c = piece_of(r, from);
     asm volatile(
@@ -718,9 +719,10 @@ __device__ __forceinline__ uint32_t bulk_in(const RowTensor& r, int64_t b, uint3
   return bytes;
 }
 
-__device__ __forceinline__ void bulk_out(const RowTensor& r, int64_t b, uint32_t at, uint32_t lane, uint32_t lanes) {
+__device__ __forceinline__ void bulk_out(const RowTensor& r, int64_t b, uint32_t at, uint32_t issuer,
+                                         uint32_t issuers) {
   char* q = r.out + b * r.out_row;
-  for (uint32_t s = lane; s < r.n_seg; s += lanes) {
+  for (uint32_t s = issuer; s < r.n_seg; s += issuers) {
     char* to = q + s * r.out_seg;
     const Piece c = piece_of(r, to);
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + c.lead),
@@ -959,12 +961,12 @@ __device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, 
 // G threads for each element, whose slices are staged in shared memory: global
 // memory is read once and written once. CLUSTER: the blocks of a cluster share
 // one element. Bound by DRAM for elements of some KB and more: B = 65536, T = 50
-// time-major 879 us for 5.5 GB (6.27 TB/s, 96 % of the copy rate); B = 16384,
+// time-major 869 us for 5.5 GB (6.34 TB/s, 97 % of the copy rate); B = 16384,
 // T = 20 95 us time-major, 86 us batch-major for 552 MB; the 13-state model,
-// B = 4096, T = 20 35 us for 201 MB. What the time-major layout costs is not its
-// segments' half sectors: pairs of elements, whose segments have none, take as
-// long. Shorter elements are bound by instructions: B = 16384 sigmoid rows of
-// 2.3 KB 15.0 us for 75 MB.
+// B = 4096, T = 20 33 us for 201 MB. What the time-major layout costs it costs in
+// writing (reading alone 112 us against 109, T = 50, 0.8 GB; with writing 250
+// against 230), and the more the more segments an element has. Shorter elements
+// are bound by instructions: B = 16384 sigmoid rows of 2.3 KB 14.7 us for 75 MB.
 template <int G, int THREADS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
     grad_rows_kernel(const __grid_constant__ RowTable tab) {
@@ -973,7 +975,10 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
   __shared__ uint64_t bars[THREADS / G];
   __shared__ RowTensor parts[CLUSTER ? ROW_MAX_TENSORS : 1];
   constexpr int PER = THREADS / G;
-  constexpr uint32_t LANES = G < 32 ? G : 32;  // that issue bulk copies
+  // Every thread issues bulk copies, neighbouring segments by different warps: a
+  // warp issues those of its lanes one after the other (one warp for all: reading
+  // 0.8 GB of 784-byte segments took 137 us instead of 112).
+  constexpr uint32_t WARPS = G > 32 ? G / 32 : 1;
   const uint32_t group = threadIdx.x / G, lane = threadIdx.x % G;
   int64_t b = (int64_t)blockIdx.x * PER + group;
   uint32_t staged_bytes = tab.staged_bytes;
@@ -998,15 +1003,16 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
   char* mine = staged + group * staged_bytes;
   const uint32_t to = smem_u32(mine);
   uint64_t* bar = bars + group;
-  if (tab.bulk && lane < LANES) {
+  const uint32_t issuer = lane % 32 * WARPS + lane / 32;
+  if (tab.bulk) {
     if (lane == 0) {
-      mbar_init(bar, LANES);
+      mbar_init(bar, G);
       fence_mbar_init();
     }
-    __syncwarp(group_mask<G>());
+    group_sync<G>();
     uint32_t bytes = 0;
     for (int k = 0; k < tab.n; ++k)
-      if (tensors[k].bulk) bytes += bulk_in(tensors[k], b, to + tensors[k].staged, bar, lane, LANES);
+      if (tensors[k].bulk) bytes += bulk_in(tensors[k], b, to + tensors[k].staged, bar, issuer, G);
     mbar_expect_tx(bar, bytes);
   }
   for (int k = 0; k < tab.n; ++k) {
@@ -1056,10 +1062,10 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
     fence_proxy_async();
     group_sync<G>();
   }
-  if (tab.bulk && lane < LANES) {
+  if (tab.bulk) {
     for (int k = 0; k < tab.n; ++k) {
       const RowTensor& r = tensors[k];
-      if (r.bulk && (changed || r.in != r.out)) bulk_out(r, b, to + r.staged, lane, LANES);
+      if (r.bulk && (changed || r.in != r.out)) bulk_out(r, b, to + r.staged, issuer, G);
     }
     bulk_commit();
   }
@@ -1075,8 +1081,8 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
     else if (r.vec_bytes == 4) threads_out<4>(r, b, mine + r.staged, lane, G);
     else threads_out<2>(r, b, mine + r.staged, lane, G);
   }
-  if (tab.bulk && lane < LANES) bulk_wait_read<0>();  // the copies read this block's memory
-  if constexpr (CLUSTER) cluster_wait();              // and the cluster's blocks their sums
+  if (tab.bulk) bulk_wait_read<0>();      // the copies read this block's memory
+  if constexpr (CLUSTER) cluster_wait();  // and the cluster's blocks their sums
 }
 
 // Elements that shared memory cannot hold: both passes read global memory.
@@ -1225,6 +1231,8 @@ size_t part_bytes(const RowTable& tab, size_t parts) {
   return bytes;
 }
 
+// cluster: blocks of a cluster, which share an element (CLUSTER) or have one each
+// and are together only to run on neighbouring SMs.
 template <int G, int THREADS, bool CLUSTER = false>
 cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned cluster = 1) {
   constexpr int PER = THREADS / G;
@@ -1241,7 +1249,8 @@ cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned clust
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((tab.B + PER - 1) / PER) * cluster);
+  const int64_t blocks = CLUSTER ? tab.B * cluster : (tab.B + PER - 1) / PER;
+  cfg.gridDim = dim3((unsigned)((blocks + cluster - 1) / cluster * cluster));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1249,7 +1258,7 @@ cudaError_t launch_rows(const RowTable& tab, cudaStream_t stream, unsigned clust
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim = {cluster, 1, 1};
   cfg.attrs = &attr;
-  cfg.numAttrs = CLUSTER ? 1 : 0;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, tab);
 }
 
@@ -1259,7 +1268,7 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // Threads for an element by what it stages. More threads cost instructions
   // that every element repeats (its records, the join, square root and quotient),
   // fewer leave the additions of long elements to few: us by threads, bytes of an
-  // element and number of elements:
+  // element and number of elements (without the pairs below):
   //     bytes (elements)    4     8    16    32    64   128
   //       266 (100000)     15    19    32    55   122   212
   //       602  (60000)     17    18    25    40    83   135
@@ -1275,10 +1284,14 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   if (tab.staged_bytes <= 4096) return launch_rows<16, 128>(tab, stream);
   if (tab.staged_bytes <= 12288) return launch_rows<32, 128>(tab, stream);
   if (tab.staged_bytes <= 20480) return launch_rows<64, 64>(tab, stream);
-  if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream);
+  // Blocks of neighbouring elements in pairs, whose segments' ends meet in a line
+  // of L2: with up to twelve of them on an SM 42042 bytes 887 -> 869 us, 24534
+  // time-major 48.5 -> 44.6, batch-major 35.0 -> 33.4; with more (16842 bytes) the
+  // scheduling of pairs costs more than that, 95 -> 110.
+  if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream, 2);
   // Longer ones leave an SM one or two blocks, whose copies, sums and stores
   // take turns: blocks of a cluster share them. us in one block | 2 | 4 | 8:
-  //  84042 (2048)  91 | 82 | 92 | 137      210042 (1024)  162 | 126 | 110 | 108
+  //  84042 (2048)  91 | 77 | 92 | 137      210042 (1024)  162 | 126 | 101 | 108
   if (tab.B <= INT32_MAX / 8)
     for (unsigned parts = 2; parts <= 8; parts *= 2)
       if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
