@@ -1269,16 +1269,18 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // that every element repeats (its records, the join, square root and quotient),
   // fewer leave the additions of long elements to few: us by threads, bytes of an
   // element and number of elements (without the pairs below):
-  //     bytes (elements)    4     8    16    32    64   128
-  //       266 (100000)     15    19    32    55   122   212
-  //       602  (60000)     17    18    25    40    83   135
-  //      1722  (40000)     30    26    28    39    78   128
-  //      2282  (65536)           49    49    52
-  //      4242  (16384)           37    28    27    40    61
-  //      8442  (16384)           82    57    49    52    72
-  //     16842  (16384)                 112   87    87    86
-  //     24534   (4096)                  92   64    53    49
-  //     42042  (65536)                     1030   930   880
+  //     bytes (elements)    4     8    16    32    64   128   256
+  //       266 (100000)     15    19    31    55   120   205
+  //       602  (60000)     16    18    25    40    82   141
+  //      1722  (40000)     30    25    28    39    75   129
+  //      2282  (65536)     53    49    48    52    93   161
+  //      4242  (16384)     40    36    28    27    39    60
+  //      8442  (16384)    117    82    58    49    49    70   129
+  //     16842  (16384)                 113    86    86    86   121
+  //     24534   (4096)                  93    64    52    49    56
+  //     42042  (65536)                      1409   877   887   873
+  //     84042   (2048)                              92    76    72
+  //    210042   (1024)                             157   119   111
   if (tab.staged_bytes <= 640) return launch_rows<4, 64>(tab, stream);
   if (tab.staged_bytes <= 2048) return launch_rows<8, 128>(tab, stream);
   if (tab.staged_bytes <= 4096) return launch_rows<16, 128>(tab, stream);
@@ -1289,9 +1291,10 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // time-major 48.5 -> 44.6, batch-major 35.0 -> 33.4; with more (16842 bytes) the
   // scheduling of pairs costs more than that, 95 -> 110.
   if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream, 2);
-  // Longer ones leave an SM one or two blocks, whose copies, sums and stores
-  // take turns: blocks of a cluster share them. us in one block | 2 | 4 | 8:
-  //  84042 (2048)  91 | 77 | 92 | 137      210042 (1024)  162 | 126 | 101 | 108
+  if (tab.staged_bytes <= 114688) return launch_rows<256, 256>(tab, stream);
+  // Longer ones leave an SM one block, whose copies, sums and stores take turns:
+  // blocks of a cluster share them. us in one block | 2 | 4 | 8:
+  //  84042 (2048)  72 | 79 | 90 | 134      210042 (1024)  111 | 105 | 103 | 104
   if (tab.B <= INT32_MAX / 8)
     for (unsigned parts = 2; parts <= 8; parts *= 2)
       if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
