@@ -1214,6 +1214,7 @@ cudaError_t launch_grad_small(const GradTable<CAP>& tab, bool max_type, const Gr
 template cudaError_t launch_grad_small<GRAD_CAP_SHORT>(const GradTable<GRAD_CAP_SHORT>&, bool, const GradScale*,
                                                        const GradNormOut&, cudaStream_t);
 INSTANTIATE(GRAD_CAP_SHORT)
+INSTANTIATE(GRAD_CAP_MIDDLE)
 INSTANTIATE(GRAD_CAP_LONG)
 #undef INSTANTIATE
 

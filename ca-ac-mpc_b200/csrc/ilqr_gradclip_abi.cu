@@ -50,30 +50,34 @@ int check_list(const List& l, int32_t norm_type) {
 
 struct Span {
   uintptr_t lo, hi;
-  int32_t tensor;
-  bool out;
 };
+
+void sort_spans(std::vector<Span>& s) {
+  const auto before = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
+}
 
 // Whether a value that the call writes is also one that it writes or reads
 // elsewhere: blocks run in no order, so only a tensor's own input may be its
 // output, whole.
 bool overlaps(const List& l) {
-  std::vector<Span> s;
-  s.reserve(2 * (size_t)l.n);
+  std::vector<Span> outs, ins;  // of those that are not in place
+  outs.reserve((size_t)l.n);
   for (int32_t i = 0; i < l.n; ++i) {
     if (l.numel[i] == 0) continue;
     const uintptr_t bytes = (uintptr_t)(l.numel[i] * size_of(l.dtype[i]));
     const uintptr_t q = (uintptr_t)l.out[i], p = (uintptr_t)l.in[i];
-    s.push_back({q, q + bytes, i, true});
-    if (p != q) s.push_back({p, p + bytes, i, false});
+    outs.push_back({q, q + bytes});
+    if (p != q) ins.push_back({p, p + bytes});
   }
-  const auto before = [](const Span& a, const Span& b) { return a.lo < b.lo; };
-  if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
-  uintptr_t end_out = 0, end_any = 0;  // of the spans before this one
-  for (const Span& x : s) {
-    if (x.lo < (x.out ? end_any : end_out)) return true;
-    end_any = std::max(end_any, x.hi);
-    if (x.out) end_out = std::max(end_out, x.hi);
+  sort_spans(outs);
+  for (size_t k = 1; k < outs.size(); ++k)
+    if (outs[k].lo < outs[k - 1].hi) return true;
+  sort_spans(ins);
+  size_t k = 0;
+  for (const Span& x : ins) {
+    while (k < outs.size() && outs[k].hi <= x.lo) ++k;
+    if (k < outs.size() && outs[k].lo < x.hi) return true;
   }
   return false;
 }
@@ -226,8 +230,9 @@ int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const in
     double* slots = static_cast<double*>(workspace);
     const bool mx = norm_type == ILQR_NORM_MAX;
     if (tensor_norms == nullptr && is_small(l)) return small_impl(l, mx, nullptr, o, stream);
-    return n_tensors <= ilqr::GRAD_CAP_SHORT ? norm_impl<ilqr::GRAD_CAP_SHORT>(l, mx, o, slots, stream)
-                                             : norm_impl<ilqr::GRAD_CAP_LONG>(l, mx, o, slots, stream);
+    if (n_tensors <= ilqr::GRAD_CAP_SHORT) return norm_impl<ilqr::GRAD_CAP_SHORT>(l, mx, o, slots, stream);
+    if (n_tensors <= ilqr::GRAD_CAP_MIDDLE) return norm_impl<ilqr::GRAD_CAP_MIDDLE>(l, mx, o, slots, stream);
+    return norm_impl<ilqr::GRAD_CAP_LONG>(l, mx, o, slots, stream);
   } catch (...) {
     return ILQR_ERR_HOST_MEMORY;
   }
@@ -255,8 +260,9 @@ int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_
     if (overlaps(l)) return ILQR_ERR_OVERLAP;
     if (total == nullptr && is_small(l))
       return small_impl(l, s.max_type != 0, &s, ilqr::GradNormOut{norm, nullptr, nullptr}, stream);
-    return n_tensors <= ilqr::GRAD_CAP_SHORT ? clip_impl<ilqr::GRAD_CAP_SHORT>(l, s, total, norm, slots, stream)
-                                             : clip_impl<ilqr::GRAD_CAP_LONG>(l, s, total, norm, slots, stream);
+    if (n_tensors <= ilqr::GRAD_CAP_SHORT) return clip_impl<ilqr::GRAD_CAP_SHORT>(l, s, total, norm, slots, stream);
+    if (n_tensors <= ilqr::GRAD_CAP_MIDDLE) return clip_impl<ilqr::GRAD_CAP_MIDDLE>(l, s, total, norm, slots, stream);
+    return clip_impl<ilqr::GRAD_CAP_LONG>(l, s, total, norm, slots, stream);
   } catch (...) {
     return ILQR_ERR_HOST_MEMORY;
   }

@@ -202,7 +202,7 @@ def test_bounds_at_their_ends():
     assert torch.isnan(got[0]).all()
 
 
-@pytest.mark.parametrize("count", [59, 60, 61, 1000, 1001, 5003])
+@pytest.mark.parametrize("count", [59, 60, 61, 240, 241, 1000, 1001, 5003])
 def test_many_tensors(count):
     """Lists beyond what one launch takes, of mixed types and sizes."""
     rng = np.random.default_rng(count)

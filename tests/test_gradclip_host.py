@@ -84,6 +84,10 @@ def test_clip_refusals():
     assert _clip(out=(2 * A, 4 * A)) == 7                      # the other's input
     assert _clip(out=(3 * A, 3 * A + 16), numel=(5, 7)) == 7   # 20 bytes, then 4 of them again
     assert _clip(grads=(A, 2 * A), out=(A, 3 * A), numel=((2 * A - A) // 4 + 1, 7)) == 7
+    # far from its own output, and within a long one of another tensor, in either order
+    assert _clip(grads=(A, 5 * A + 400), out=(5 * A, 9 * A), numel=(1000, 7)) == 7
+    assert _clip(grads=(5 * A + 400, A), out=(9 * A, 5 * A), numel=(7, 1000)) == 7
+    assert _clip(grads=(A, 5 * A + 3996), out=(5 * A, 9 * A), numel=(1000, 7)) == 7
 
 
 def test_elements_refusals():
