@@ -30,7 +30,8 @@ namespace ilqr {
 
 namespace {
 
-constexpr int BLK = 256;  // threads of a block
+constexpr int BLK = 256;        // threads of a block
+constexpr int LONG_BLK = 1024;  // and of one that shares an element beyond shared memory
 constexpr int UN = 4;     // 16-byte loads that a thread has in flight
 
 // ---- values ----------------------------------------------------------------
@@ -1085,19 +1086,23 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
   if constexpr (CLUSTER) cluster_wait();  // and the cluster's blocks their sums
 }
 
-// Elements that shared memory cannot hold: both passes read global memory.
-__global__ void __launch_bounds__(BLK) grad_long_rows_kernel(const __grid_constant__ RowTable tab) {
-  __shared__ double sh[32];
-  const int64_t b = blockIdx.x;
-  const uint32_t lane = threadIdx.x;
+// Elements that the shared memory of a cluster cannot hold: its blocks share one,
+// and both passes read global memory. 64 elements of 2.8 MB 100 us, 300 of 2 MB
+// 312 us (3.9 TB/s of what must move); a single one of 52 MB 248 us, what eight SMs
+// can read and write.
+__global__ void __launch_bounds__(LONG_BLK) grad_long_rows_kernel(const __grid_constant__ RowTable tab) {
+  __shared__ double sh[33];
+  const uint32_t n_blocks = cluster_size();
+  const int64_t b = blockIdx.x / n_blocks;
+  const uint32_t lane = cluster_rank() * LONG_BLK + threadIdx.x, step = n_blocks * LONG_BLK;
   Acc<false> a;
   for (int k = 0; k < tab.n; ++k) {
     const RowTensor& r = tab.t[k];
-#define CALL(DT, VB) row_sum<DT, VB>(a, r, b, lane, BLK)
+#define CALL(DT, VB) row_sum<DT, VB>(a, r, b, lane, step)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
-  const double nrm = sqrt(block_join<false>(a.s, sh));
+  const double nrm = sqrt(cluster_join<false>(block_join<false>(a.s, sh), sh + 32));
   if (lane == 0 && tab.norms != nullptr) tab.norms[b] = (float)nrm;
   const Coef c = coef_of(nrm, tab.max_norm, tab.eps);
   const bool zero = tab.zero_nonfinite && !isfinite(nrm);
@@ -1105,13 +1110,14 @@ __global__ void __launch_bounds__(BLK) grad_long_rows_kernel(const __grid_consta
     const RowTensor& r = tab.t[k];
     if (c.d == 1.0 && !zero && r.in == r.out) continue;
     if (zero || c.wide) {
-      row_apart(r, b, c, zero, lane, BLK);
+      row_apart(r, b, c, zero, lane, step);
       continue;
     }
-#define CALL(DT, VB) row_scale<DT, VB>(r, b, c, lane, BLK)
+#define CALL(DT, VB) row_scale<DT, VB>(r, b, c, lane, step)
     ROW_DISPATCH(r, CALL)
 #undef CALL
   }
+  cluster_wait();
 }
 
 // ---- launches ---------------------------------------------------------------
@@ -1296,11 +1302,19 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // Longer ones leave an SM one block, whose copies, sums and stores take turns:
   // blocks of a cluster share them. us in one block | 2 | 4 | 8:
   //  84042 (2048)  72 | 79 | 90 | 134      210042 (1024)  111 | 105 | 103 | 104
-  if (tab.B <= INT32_MAX / 8)
-    for (unsigned parts = 2; parts <= 8; parts *= 2)
-      if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
-        return launch_rows<128, 128, true>(tab, stream, parts);
-  return launch(grad_long_rows_kernel, (unsigned)tab.B, false, stream, tab);
+  for (unsigned parts = 2; parts <= 8; parts *= 2)
+    if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
+      return launch_rows<128, 128, true>(tab, stream, parts);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tab.B * 8);
+  cfg.blockDim = dim3(LONG_BLK);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {8, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, grad_long_rows_kernel, tab);
 }
 
 }  // namespace ilqr
