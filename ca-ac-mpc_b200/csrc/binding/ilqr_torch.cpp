@@ -4,8 +4,8 @@
 // types and strides are read here: the same reading through the Python
 // interface costs 0.6 us a tensor and takes longer than the kernels for most
 // lists (400 bf16 tensors of 600 MB: 246 us against 113 us of GPU time). The
-// checks and errors are those of ilqr_native.py, which documents the calls;
-// everything else goes through the C ABI in include/ilqr_b200.h.
+// calls are documented in ilqr_native.py; everything but the reading goes through
+// the C ABI in include/ilqr_b200.h.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -75,6 +75,49 @@ void read_list(PyObject* list, Tensors& out) {
   }
 }
 
+// What a caller gave for a list of tensors, as a Python list.
+PyObject* as_list(PyObject* given, const char* name) {
+  TORCH_CHECK_TYPE(!THPVariable_Check(given), name, " must be a sequence of tensors, not one tensor");
+  if (PyList_CheckExact(given)) {
+    Py_INCREF(given);
+    return given;
+  }
+  return PySequence_List(given);
+}
+
+// The outputs a caller gave as a new Python list; None stays.
+PyObject* given_outputs(PyObject* given) {
+  if (given == Py_None) return Py_NewRef(given);
+  TORCH_CHECK_TYPE(!THPVariable_Check(given), "out must be a sequence of tensors, not one tensor");
+  return PySequence_List(given);
+}
+
+bool truth(PyObject* o) {
+  const int t = PyObject_IsTrue(o);
+  if (t < 0) throw python_error();
+  return t == 1;
+}
+
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+int32_t norm_code(PyObject* norm_type) {
+  const double p = number(norm_type);
+  TORCH_CHECK_VALUE(p == 2.0 || p == INFINITY, "norm_type must be 2 or inf, not ", p);
+  return p == 2.0 ? ILQR_NORM_L2 : ILQR_NORM_MAX;
+}
+
+struct Bound {
+  double max_norm, eps;
+  Bound(PyObject* m, PyObject* e) : max_norm(number(m)), eps(number(e)) {
+    TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative or NaN, got ", max_norm);
+    TORCH_CHECK_VALUE(eps >= 0.0 && eps < INFINITY, "eps must be finite and not negative, got ", eps);
+  }
+};
+
 struct Dim {
   int64_t size, stride;
 };
@@ -119,8 +162,8 @@ at::Tensor gathered(const at::Tensor& t) {
   return flat;
 }
 
-// The outputs as a new Python list: new tensors, or `given` checked against
-// the inputs.
+// The outputs: a Python list of new tensors, or `given` (of given_outputs)
+// checked against the inputs.
 PyObject* outputs(PyObject* given, PyObject* grads_list, const Tensors& grads, Tensors& out) {
   const Py_ssize_t n = (Py_ssize_t)grads.size();
   out.reserve((size_t)n);
@@ -134,12 +177,10 @@ PyObject* outputs(PyObject* given, PyObject* grads_list, const Tensors& grads, T
     }
     return list.release();
   }
-  TORCH_CHECK_TYPE(!THPVariable_Check(given), "out must be a sequence of tensors, not one tensor");
-  Object list(PySequence_List(given));
-  TORCH_CHECK(PyList_GET_SIZE(list.p) == n, "out must hold ", n, " tensors, got ", PyList_GET_SIZE(list.p));
+  TORCH_CHECK(PyList_GET_SIZE(given) == n, "out must hold ", n, " tensors, got ", PyList_GET_SIZE(given));
   const bool grad_mode = at::GradMode::is_enabled();
   for (Py_ssize_t i = 0; i < n; ++i) {
-    PyObject* o = PyList_GET_ITEM(list.p, i);
+    PyObject* o = PyList_GET_ITEM(given, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), "out must hold tensors, not ", Py_TYPE(o)->tp_name);
     const at::Tensor& t = THPVariable_Unpack(o);
     if (o != PyList_GET_ITEM(grads_list, i)) {
@@ -153,7 +194,7 @@ PyObject* outputs(PyObject* given, PyObject* grads_list, const Tensors& grads, T
     TORCH_CHECK(one_to_a_place(t), "out must hold tensors whose values each have a place of their own");
     out.push_back(t);
   }
-  return list.release();
+  return Py_NewRef(given);
 }
 
 void written(const Tensors& out) {
@@ -188,14 +229,16 @@ at::Tensor workspace(int32_t n, c10::Device device, size_t* bytes) {
   return new_tensor({(int64_t)*bytes}, at::kByte, device);
 }
 
-// grad_norm(grads: list, norm code, norm?, norms?, total?) -> tuple of those asked for
+// grad_norm(grads, norm_type, norm?, norms?, total?) -> tuple of those asked for
 PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(nargs == 5 && PyList_Check(args[0]), "grad_norm takes a list and four numbers");
-  const int32_t code = (int32_t)PyLong_AsLong(args[1]);
-  const bool want[3] = {args[2] == Py_True, args[3] == Py_True, args[4] == Py_True};
+  TORCH_CHECK_TYPE(nargs == 5, "grad_norm takes five values");
+  const int32_t code = norm_code(args[1]);
+  bool want[3];
+  for (int k = 0; k < 3; ++k) want[k] = truth(args[2 + k]);
+  const Object given(as_list(args[0], "grads"));
   Tensors grads;
-  read_list(args[0], grads);
+  read_list(given.p, grads);
   TORCH_CHECK(!grads.empty(), "grads is empty: there is no device to put its norm on");
   at::NoGradGuard no_grad;
   const c10::Device device = grads[0].device();
@@ -235,14 +278,17 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// clip_grad_norm(grads: list, out or None, max_norm, norm code, eps, total or None) -> (out, norm)
+// clip_grad_norm(grads, out or None, max_norm, norm_type, eps, total or None) -> (out, norm)
 PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(nargs == 6 && PyList_Check(args[0]), "clip_grad_norm takes a list and five values");
-  const double max_norm = PyFloat_AsDouble(args[2]), eps = PyFloat_AsDouble(args[4]);
-  const int32_t code = (int32_t)PyLong_AsLong(args[3]);
+  TORCH_CHECK_TYPE(nargs == 6, "clip_grad_norm takes six values");
+  const int32_t code = norm_code(args[3]);
+  const Bound bound(args[2], args[4]);
+  // all that may run the caller's code comes before the first tensor is read
+  const Object given_out(given_outputs(args[1]));
+  const Object given(as_list(args[0], "grads"));
   Tensors grads, out;
-  read_list(args[0], grads);
+  read_list(given.p, grads);
   TORCH_CHECK(!grads.empty(), "grads is empty: there is no device to put its norm on");
   const c10::Device device = grads[0].device();
   const double* total = nullptr;
@@ -256,7 +302,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const c10::cuda::OptionalCUDAGuard guard(device);
   device_ok(device.index());
-  Object list(outputs(args[1], args[0], grads, out));
+  Object list(outputs(given_out.p, given.p, grads, out));
   at::NoGradGuard no_grad;
   const int32_t n = (int32_t)grads.size();
   Arrays a;
@@ -276,7 +322,8 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor norm = new_tensor({}, at::kFloat, device);
   size_t bytes = 0;
   const at::Tensor ws = workspace(n, device, &bytes);
-  check(ilqr_b200_grad_clip(a.in.data(), to.data(), a.numel.data(), a.types.data(), n, code, max_norm, eps, total,
+  check(ilqr_b200_grad_clip(a.in.data(), to.data(), a.numel.data(), a.types.data(), n, code, bound.max_norm, bound.eps,
+                            total,
                             norm.mutable_data_ptr<float>(), ws.mutable_data_ptr(), bytes,
                             c10::cuda::getCurrentCUDAStream(device.index()).stream()),
         "ilqr_b200_grad_clip");
@@ -317,23 +364,27 @@ bool segments(const at::Tensor& g, const at::Tensor& o, int64_t d, int64_t* lay)
   return true;
 }
 
-// clip_grad_elements(grads: list, out or None, batch dims: int or list, max_norm, eps, zero?) -> (out, norms)
+// clip_grad_elements(grads, out or None, batch dims: a number or a sequence, max_norm, eps, zero?) -> (out, norms)
 PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(nargs == 6 && PyList_Check(args[0]), "clip_grad_elements takes a list and five values");
-  const double max_norm = PyFloat_AsDouble(args[3]), eps = PyFloat_AsDouble(args[4]);
+  TORCH_CHECK_TYPE(nargs == 6, "clip_grad_elements takes six values");
+  const Bound bound(args[3], args[4]);
+  const bool zero_nonfinite = truth(args[5]);
+  const bool each = !PyLong_Check(args[2]);
+  const Object given_out(given_outputs(args[1]));
+  const Object given_dims(each ? PySequence_List(args[2]) : Py_NewRef(args[2]));
+  const Object given(as_list(args[0], "grads"));
   Tensors grads, out;
-  read_list(args[0], grads);
+  read_list(given.p, grads);
   const size_t n = grads.size();
   TORCH_CHECK(n >= 1 && n <= ILQR_MAX_ELEMENT_TENSORS, "grads must hold 1 to ", ILQR_MAX_ELEMENT_TENSORS,
               " tensors, got ", n);
   int64_t dims[ILQR_MAX_ELEMENT_TENSORS];
-  const bool each = PyList_Check(args[2]);
-  TORCH_CHECK(!each || (size_t)PyList_GET_SIZE(args[2]) == n, "batch_dims must hold ", n, " numbers, got ",
-              each ? PyList_GET_SIZE(args[2]) : 0);
+  TORCH_CHECK(!each || (size_t)PyList_GET_SIZE(given_dims.p) == n, "batch_dims must hold ", n, " numbers, got ",
+              each ? PyList_GET_SIZE(given_dims.p) : 0);
   int64_t B = 0;
   for (size_t i = 0; i < n; ++i) {
-    dims[i] = PyLong_AsLongLong(each ? PyList_GET_ITEM(args[2], i) : args[2]);
+    dims[i] = PyLong_AsLongLong(each ? PyList_GET_ITEM(given_dims.p, i) : given_dims.p);
     if (dims[i] == -1 && PyErr_Occurred()) throw python_error();
     TORCH_CHECK(dims[i] >= 0 && dims[i] < grads[i].dim(), "batch dimension ", dims[i], " of a tensor of shape ",
                 grads[i].sizes());
@@ -344,7 +395,7 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   const c10::Device device = grads[0].device();
   const c10::cuda::OptionalCUDAGuard guard(device);
   device_ok(device.index());
-  Object list(outputs(args[1], args[0], grads, out));
+  Object list(outputs(given_out.p, given.p, grads, out));
   at::NoGradGuard no_grad;
   Arrays a;
   Small<void*> to;
@@ -364,8 +415,8 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     }
   }
   const at::Tensor norms = new_tensor({B}, at::kFloat, device);
-  check(ilqr_b200_grad_clip_elements(a.in.data(), to.data(), a.types.data(), layout, (int32_t)n, B, max_norm, eps,
-                                     args[5] == Py_True ? 1 : 0, norms.mutable_data_ptr<float>(),
+  check(ilqr_b200_grad_clip_elements(a.in.data(), to.data(), a.types.data(), layout, (int32_t)n, B, bound.max_norm,
+                                     bound.eps, zero_nonfinite ? 1 : 0, norms.mutable_data_ptr<float>(),
                                      c10::cuda::getCurrentCUDAStream(device.index()).stream()),
         "ilqr_b200_grad_clip_elements");
   for (const auto& b : back) out[b.first].copy_(b.second);

@@ -13,7 +13,6 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
-import math
 import os
 import threading
 from typing import Optional, Sequence
@@ -966,7 +965,6 @@ def fastmpc_assembly(K, k, v0, A, Bm, X, U, x_ref=None, u_ref=None, compute_xref
 # too (csrc/binding/ilqr_torch.cpp, built beside the library).
 
 BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "ilqr_torch.so")
-MAX_ELEMENT_TENSORS = 8
 _binding_module = None
 
 
@@ -987,36 +985,12 @@ def _binding():
     return _binding_module
 
 
-def _as_list(tensors, name):
-    if isinstance(tensors, torch.Tensor):
-        raise TypeError(f"{name} must be a sequence of tensors, not one tensor")
-    return tensors if type(tensors) is list else list(tensors)
-
-
-def _norm_code(norm_type) -> int:
-    if norm_type == 2:
-        return 0
-    if norm_type == math.inf:
-        return 1
-    raise ValueError(f"norm_type must be 2 or inf, not {norm_type!r}")
-
-
-def _bound(max_norm, eps):
-    max_norm, eps = float(max_norm), float(eps)
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
-    return max_norm, eps
-
-
 def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False):
     """Norm over all values of a sequence of gradients (float32, float16 or
     bfloat16, mixed as they come, any strides), a 0-d float32 tensor on their
     device; with per_tensor also each tensor's own norm, [n]. norm_type 2 or
     inf. Nothing is read back to the host."""
-    code = _norm_code(norm_type)
-    got = _binding().grad_norm(_as_list(grads, "grads"), code, True, bool(per_tensor), False)
+    got = (_binding_module or _binding()).grad_norm(grads, norm_type, True, per_tensor, False)
     return got if per_tensor else got[0]
 
 
@@ -1024,8 +998,7 @@ def grad_norm_total(grads, norm_type: float = 2.0):
     """What grad_norm takes the norm of, a 0-d float64 tensor: the sum of
     squares, or for inf the largest magnitude. Totals of lists on several
     devices are added (or the largest taken) and given to clip_grad_norm."""
-    code = _norm_code(norm_type)
-    return _binding().grad_norm(_as_list(grads, "grads"), code, False, False, True)[0]
+    return (_binding_module or _binding()).grad_norm(grads, norm_type, False, False, True)[0]
 
 
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 1e-6, total=None, out=None):
@@ -1036,9 +1009,7 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 
     place. No output may share memory with another tensor of the call. A bound
     of inf changes nothing; a NaN norm makes every value NaN, an infinite one 0
     or NaN. The outputs carry no autograd history."""
-    code = _norm_code(norm_type)
-    max_norm, eps = _bound(max_norm, eps)
-    return _binding().clip_grad_norm(_as_list(grads, "grads"), out, max_norm, code, eps, total)
+    return (_binding_module or _binding()).clip_grad_norm(grads, out, max_norm, norm_type, eps, total)
 
 
 def clip_grad_elements(grads, max_norm: float, batch_dims=0, eps: float = 1e-6, zero_nonfinite: bool = False, out=None):
@@ -1051,8 +1022,4 @@ def clip_grad_elements(grads, max_norm: float, batch_dims=0, eps: float = 1e-6, 
     own become NaN (or 0, where its norm is infinite), or with zero_nonfinite
     zero. Returns (the scaled gradients, norms [B] float32); out as in
     clip_grad_norm."""
-    max_norm, eps = _bound(max_norm, eps)
-    if not isinstance(batch_dims, int):
-        batch_dims = [int(d) for d in batch_dims]
-    return _binding().clip_grad_elements(_as_list(grads, "grads"), out, batch_dims, max_norm, eps,
-                                         bool(zero_nonfinite))
+    return (_binding_module or _binding()).clip_grad_elements(grads, out, batch_dims, max_norm, eps, zero_nonfinite)

@@ -140,6 +140,22 @@ def test_binding_refusals_without_gpu():
         nat.clip_grad_elements([x], 1.0)
     with pytest.raises(ValueError, match="max_norm"):
         nat.clip_grad_elements([x], math.nan)
+    with pytest.raises(TypeError):
+        nat.clip_grad_norm([x], "one")
+    with pytest.raises(TypeError):
+        nat.clip_grad_norm([x], 1.0, out=x)
+    with pytest.raises(TypeError):
+        nat.clip_grad_elements([x], 1.0, batch_dims=1.5)
+    with pytest.raises(TypeError):
+        nat.grad_norm(3)
+
+    def fails():
+        yield x
+        raise KeyError("the caller's own")
+    for call in (lambda: nat.grad_norm(fails()), lambda: nat.clip_grad_norm([x], 1.0, out=fails()),
+                 lambda: nat.clip_grad_elements([x], 1.0, batch_dims=(1 // 0 for _ in range(1)))):
+        with pytest.raises((KeyError, ZeroDivisionError)):
+            call()
 
 
 # ---- the paths' host logic ---------------------------------------------------
