@@ -673,9 +673,6 @@ template <int VB>
 __device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
   if constexpr (VB == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  } else if constexpr (VB == 2) {
-    const uint16_t w = *reinterpret_cast<const uint16_t*>(from);
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(w) : "memory");
   } else {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(VB) : "memory");
   }
@@ -732,26 +729,38 @@ __device__ __forceinline__ void bulk_out(const RowTensor& r, int64_t b, uint32_t
   }
 }
 
-// The ends of the segments: the first word of a place and the last three hold
-// all that the bulk copies leave.
+// The ends of the segments, one for each thread: the first word of a place, where
+// the segment begins within it, and what follows the last whole one.
 template <int VB, bool OUT>
 __device__ __forceinline__ void ends(const RowTensor& r, int64_t b, char* staged, uint32_t lane, uint32_t step) {
-  constexpr uint32_t PER = 64 / VB;
+  constexpr uint32_t N = 16 / VB;
   char* g = OUT ? r.out + b * r.out_row : const_cast<char*>(r.in) + b * r.in_row;
   const int64_t seg = OUT ? r.out_seg : r.in_seg;
-  for (uint32_t i = lane; i < r.n_seg * PER; i += step) {
-    const uint32_t s = i / PER, u = (i % PER) * VB;
+  for (uint32_t i = lane; i < 2 * r.n_seg; i += step) {
+    const uint32_t s = i >> 1;
     char* q = g + s * seg;
     const Piece c = piece_of(r, q);
-    const uint32_t at = u < 16 ? u : r.place - 64 + u;
-    if (at - (c.off + c.lead) < c.whole) continue;
-    const bool inside = at - c.off < r.seg_bytes;
-    Vec<VB>* mine = reinterpret_cast<Vec<VB>*>(staged + s * r.place + at);
-    Vec<VB>* theirs = reinterpret_cast<Vec<VB>*>(q + (int64_t)at - c.off);
+    const bool first = (i & 1) == 0;
+    if (first && c.lead == 0) continue;  // it begins with a whole word
+    const uint32_t at = first ? 0 : c.off + c.lead + c.whole;
+    const uint32_t from = first ? c.off : 0, to = first ? 16 : c.off + r.seg_bytes - at;
+    char* mine = staged + s * r.place + at;
+    char* theirs = q + ((int64_t)at - c.off);
+    __align__(16) Vec<VB> w[N];
     if constexpr (OUT) {
-      if (inside) *theirs = *mine;
+      if (from < to) *reinterpret_cast<Vec<16>*>(w) = load_vec<16>(mine);
+#pragma unroll
+      for (uint32_t u = 0; u < N; ++u)
+        if (u * VB >= from && u * VB < to) *reinterpret_cast<Vec<VB>*>(theirs + u * VB) = w[u];
     } else {
-      *mine = inside ? *theirs : Vec<VB>{};
+#pragma unroll
+      for (uint32_t u = 0; u < N; ++u) {
+        w[u] = Vec<VB>{};
+        if (u * VB >= from && u * VB < to) w[u] = load_vec<VB>(theirs + u * VB);
+      }
+      const uint32_t room = first ? 16 : r.place - at;
+      if (room > 0) *reinterpret_cast<Vec<16>*>(mine) = *reinterpret_cast<const Vec<16>*>(w);
+      for (uint32_t x = 16; x < room; x += 16) *reinterpret_cast<Vec<16>*>(mine + x) = Vec<16>{};
     }
   }
 }
@@ -767,7 +776,19 @@ template <int VB>
 __device__ __forceinline__ void threads_in(const RowTensor& r, int64_t b, uint32_t to, uint32_t lane, uint32_t step) {
   const char* p = r.in + b * r.in_row;
   const uint32_t n = r.n_seg * r.seg_vecs;
-  for (uint32_t i = lane; i < n; i += step) copy_async<VB>(to + i * VB, p + vec_at(r, i, VB, r.in_seg));
+  if constexpr (VB > 2) {
+    for (uint32_t i = lane; i < n; i += step) copy_async<VB>(to + i * VB, p + vec_at(r, i, VB, r.in_seg));
+  } else {  // through registers: there is no asynchronous copy of two bytes
+    for (uint32_t i = lane; i < n; i += UN * step) {
+      uint16_t w[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (i + u * step < n) w[u] = *reinterpret_cast<const uint16_t*>(p + vec_at(r, i + u * step, 2, r.in_seg));
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (i + u * step < n) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + (i + u * step) * 2), "h"(w[u]) : "memory");
+    }
+  }
 }
 
 template <int VB>
