@@ -11,6 +11,7 @@
 
 #include "ilqr_b200.h"
 #include "ilqr_gradclip.h"
+#include "ilqr_overlap.h"
 
 namespace {
 
@@ -276,8 +277,6 @@ namespace {
 struct Rows {
   uintptr_t base;
   int64_t row, seg, len, n_seg, B;
-  uintptr_t lo() const { return base; }
-  uintptr_t hi() const { return base + (uintptr_t)((B - 1) * row + (n_seg - 1) * seg + len); }
 };
 
 // Whether no two of its values share memory: one of the two strides steps over
@@ -291,16 +290,11 @@ bool apart(const Rows& r) {
   return r.row >= (r.n_seg - 1) * r.seg + r.len || r.seg >= (r.B - 1) * r.row + r.len;
 }
 
-// Whether two sets of slices share no memory. Spans that interleave are told
-// apart where both are single segments of rows with one stride (columns of
-// one packed array).
+// Whether two sets of slices share no memory: interleaved ones (columns of one
+// packed array, in either layout) are told apart.
 bool disjoint(const Rows& a, const Rows& b) {
-  if (a.hi() <= b.lo() || b.hi() <= a.lo()) return true;
-  if (a.n_seg != 1 || b.n_seg != 1 || a.row != b.row || a.B == 1) return false;
-  const Rows& x = a.base <= b.base ? a : b;
-  const Rows& y = a.base <= b.base ? b : a;
-  const int64_t at = (int64_t)((y.base - x.base) % (uintptr_t)x.row);
-  return at >= x.len && at + y.len <= x.row;
+  const ilqr::Every da[2] = {{a.B, a.row}, {a.n_seg, a.seg}}, db[2] = {{b.B, b.row}, {b.n_seg, b.seg}};
+  return !ilqr::Meeting::of({a.base, a.len, da, 2}, {b.base, b.len, db, 2});
 }
 
 // i / d = i magic >> (32 + shift) for 0 <= i < 2^31 and d >= 2: with
