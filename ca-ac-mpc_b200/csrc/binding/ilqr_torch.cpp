@@ -19,7 +19,9 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <vector>
 
+#include "../ilqr_overlap.h"
 #include "ilqr_b200.h"
 
 namespace {
@@ -197,6 +199,67 @@ PyObject* outputs(PyObject* given, PyObject* grads_list, const Tensors& grads, T
   return Py_NewRef(given);
 }
 
+using Gathered = c10::SmallVector<std::pair<size_t, at::Tensor>, 4>;
+
+// A tensor of a call, as runs of bytes.
+struct Place {
+  c10::SmallVector<ilqr::Every, 8> dims;
+  uintptr_t lo, hi;
+  int64_t len;
+  int64_t step = 0, at = 0;  // every run lies at `at` of `step` bytes; 0: not so
+  bool is_out, is_gathered;
+  Place(const at::Tensor& t, const void* p, bool o, bool g)
+      : lo((uintptr_t)p), len(t.element_size()), is_out(o), is_gathered(g) {
+    c10::SmallVector<Dim, 8> d;
+    by_stride(t, d);
+    for (const Dim& x : d) {
+      const int64_t stride = x.stride * (int64_t)t.element_size();
+      if (dims.empty() && stride == len) len *= x.size;
+      else dims.push_back({x.size, stride});
+    }
+    hi = runs().hi();
+    if (dims.empty() || dims[0].stride < len) return;
+    for (const ilqr::Every& e : dims)
+      if (e.stride % dims[0].stride != 0) return;
+    step = dims[0].stride;
+    at = (int64_t)(lo % (uintptr_t)step);
+  }
+  // Columns of one array, the usual case, without a search.
+  bool beside(const Place& x) const {
+    return step > 0 && step == x.step && at + len <= step && x.at + x.len <= step &&
+           (at + len <= x.at || x.at + x.len <= at);
+  }
+  ilqr::Strided runs() const { return {lo, len, dims.data(), (int)dims.size()}; }
+  bool is(const Place& x) const {
+    return lo == x.lo && len == x.len &&
+           std::equal(dims.begin(), dims.end(), x.dims.begin(), x.dims.end(),
+                      [](const ilqr::Every& a, const ilqr::Every& b) { return a.count == b.count && a.stride == b.stride; });
+  }
+};
+
+// The C ABI sees the copies of gathered tensors: whether what these write in the
+// end is also written, or read, elsewhere in the call is found here.
+bool gathered_overlap(const Tensors& grads, const Tensors& out, const Gathered& gathered) {
+  std::vector<Place> all;
+  all.reserve(2 * grads.size());
+  for (size_t i = 0, k = 0; i < grads.size(); ++i) {
+    const at::Tensor &g = grads[i], &o = out[i];
+    const bool there = k < gathered.size() && gathered[k].first == i;
+    if (there) ++k;
+    if (g.numel() == 0) continue;
+    all.emplace_back(o, o.mutable_data_ptr(), true, there);
+    Place in(g, g.const_data_ptr(), false, there);
+    if (!in.is(all.back())) all.push_back(std::move(in));
+  }
+  std::sort(all.begin(), all.end(), [](const Place& a, const Place& b) { return a.lo < b.lo; });
+  for (size_t a = 0; a < all.size(); ++a)
+    for (size_t b = a + 1; b < all.size() && all[b].lo < all[a].hi; ++b)
+      if ((all[a].is_out || all[b].is_out) && (all[a].is_gathered || all[b].is_gathered) &&
+          !all[a].beside(all[b]) && ilqr::Meeting::of(all[a].runs(), all[b].runs()))
+        return true;
+  return false;
+}
+
 void written(const Tensors& out) {
   for (const at::Tensor& t : out)
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -307,7 +370,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int32_t n = (int32_t)grads.size();
   Arrays a;
   Small<void*> to;
-  c10::SmallVector<std::pair<size_t, at::Tensor>, 4> back;
+  Gathered back;
   for (size_t i = 0; i < grads.size(); ++i) {
     const at::Tensor &g = grads[i], &o = out[i];
     if (without_gaps(g) && !g.is_neg() && !o.is_neg() && (g.is_same(o) || g.strides() == o.strides())) {
@@ -319,6 +382,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       to.push_back(back.back().second.mutable_data_ptr());
     }
   }
+  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back)) check(ILQR_ERR_OVERLAP, "clip_grad_norm");
   const at::Tensor norm = new_tensor({}, at::kFloat, device);
   size_t bytes = 0;
   const at::Tensor ws = workspace(n, device, &bytes);
@@ -400,7 +464,7 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   Arrays a;
   Small<void*> to;
   int64_t layout[6 * ILQR_MAX_ELEMENT_TENSORS];
-  c10::SmallVector<std::pair<size_t, at::Tensor>, 4> back;
+  Gathered back;
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor &g = grads[i], &o = out[i];
     if (!g.is_neg() && !o.is_neg() && segments(g, o, dims[i], layout + 6 * i)) {
@@ -414,6 +478,7 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       segments(flat, flat, dims[i], layout + 6 * i);
     }
   }
+  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back)) check(ILQR_ERR_OVERLAP, "clip_grad_elements");
   const at::Tensor norms = new_tensor({B}, at::kFloat, device);
   check(ilqr_b200_grad_clip_elements(a.in.data(), to.data(), a.types.data(), layout, (int32_t)n, B, bound.max_norm,
                                      bound.eps, zero_nonfinite ? 1 : 0, norms.mutable_data_ptr<float>(),

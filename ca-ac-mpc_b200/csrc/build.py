@@ -54,9 +54,9 @@ def build_binding() -> str:
     C-ABI library beside it."""
     import torch
     at = os.path.dirname(torch.__file__)
-    public = os.path.join(ROOT, "include", "ilqr_b200.h")
+    headers = [os.path.join(ROOT, "include", "ilqr_b200.h"), os.path.join(HERE, "ilqr_overlap.h")]
     # g++ as nvcc takes it (torch and this module share one libstdc++)
-    if _newer([BINDING_SRC, public, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
+    if _newer([BINDING_SRC, *headers, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
         inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
                os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
                sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]

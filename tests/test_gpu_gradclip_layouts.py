@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+import ilqr_native as nat
 from test_gpu_gradclip import DEV, F32, TYPES, _check_elements, _values
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,71 @@ def test_one_array_of_whole_elements_in_place():
     steps = p[:, 10:].unflatten(1, (T, 210))
     grads = [p[:, :10], steps[..., :196].unflatten(-1, (14, 14)), steps[..., 196:]]
     _check_elements(grads, [0, 0, 0], 20.0, out=grads)
+
+
+# ---- outputs with gaps -----------------------------------------------------------
+
+def _refused(call, *tensors):
+    """The call is refused and writes nothing."""
+    kept = [t.clone() for t in tensors]
+    with pytest.raises(RuntimeError, match="shares memory"):
+        call()
+    assert all(torch.equal(t, k) for t, k in zip(tensors, kept))
+
+
+def test_outputs_with_gaps_that_share_memory_are_refused():
+    for dtype in TYPES:
+        g, h, y = (_values((s,), dtype, k) for k, s in enumerate((50, 50, 200)))
+        other = _values((100,), dtype, 9)
+        strided = _values((100,), dtype, 8)[::2]
+        for form in (nat.clip_grad_norm, nat.clip_grad_elements):
+            # an output's gaps hold another output's values, or not
+            _refused(lambda: form([g, h], 0.5, out=[y[:100:2], y[:50]]), y)
+            _refused(lambda: form([h, g], 0.5, out=[y[:50], y[:100:2]]), y)
+            _refused(lambda: form([g, h], 0.5, out=[y[:100:2], y[98:198:2]]), y)
+            # the same gradient twice, in place
+            _refused(lambda: form([strided, strided], 0.5, out=[strided, strided]), strided)
+            # another tensor's input, and its own shifted
+            _refused(lambda: form([other[::2], y[:50]], 0.5, out=[y[1:100:2], h]), y, h)
+            _refused(lambda: form([y[:50], other[::2]], 0.5, out=[h, y[1:100:2]]), y, h)
+            _refused(lambda: form([y[:100:2]], 0.5, out=[y[2:102:2]]), y)
+        # elements whose values have two strides
+        q, out = _values((6, 8, 10), dtype, 3), torch.empty(3, 4, 5, dtype=dtype, device=DEV)
+        a, b = q[:3, :4, ::2], q[3:, 4:, ::2]
+        _refused(lambda: nat.clip_grad_elements([a, b], 0.5, out=[b, a]), q)
+        _refused(lambda: nat.clip_grad_elements([out, a], 0.5, out=[b, q[3:, 4:, :5]]), q)
+        _refused(lambda: nat.clip_grad_elements([a, out], 0.5, out=[out, q[2:5, :4, :5]]), q, out)
+        # outputs that the kernels write as they lie, over another's gathered input
+        _refused(lambda: nat.clip_grad_norm([y[:100:2], g], 0.5, out=[other[::2], y[50:100]]), y, other)
+
+
+def test_outputs_in_each_others_gaps_are_taken():
+    for dtype in TYPES:
+        for form, dims in ((nat.clip_grad_norm, ()), (nat.clip_grad_elements, (0,))):
+            g, h = _values((50,), dtype, 1), _values((50,), dtype, 2)
+            want = [t.clone() for t in form([g, h], 3.0, *dims)[0]]
+            y = torch.full((100,), 7.0, dtype=dtype, device=DEV)
+            form([g, h], 3.0, *dims, out=[y[::2], y[1::2]])
+            assert torch.equal(y[::2], want[0]) and torch.equal(y[1::2], want[1])
+            p = torch.stack([g, h], 1)
+            form([p[:, 0], p[:, 1]], 3.0, *dims, out=[p[:, 0], p[:, 1]])
+            assert torch.equal(p[:, 0], want[0]) and torch.equal(p[:, 1], want[1])
+            p = torch.stack([g, torch.full_like(g, 7.0)], 1)
+            form([p[:, 0], h], 3.0, *dims, out=[p[:, 1], h])
+            assert torch.equal(p[:, 1], want[0]) and torch.equal(p[:, 0], g) and torch.equal(h, want[1])
+            # three strides, blocks of one array
+            q = _values((6, 8, 10), dtype, 3)
+            parts = [q[:3, :4, ::2], q[:3, :4, 1::2], q[3:, 4:, :5], q[3:, :4, 5:]]
+            kept = q[:3, 4:].clone()
+            want = [t.clone() for t in form(parts, 2.0, *dims)[0]]
+            form(parts, 2.0, *dims, out=parts)
+            assert all(torch.equal(a, b) for a, b in zip(parts, want)) and torch.equal(q[:3, 4:], kept)
+
+
+def test_in_place_through_another_view():
+    """The same values seen through strides that differ where there is one step."""
+    for form in (nat.clip_grad_norm, nat.clip_grad_elements):
+        y = _values((20,), F32, 4)
+        want = form([y.as_strided((10, 1), (2, 1))], 0.1)[0][0]
+        form([y.as_strided((10, 1), (2, 1))], 0.1, out=[y.as_strided((10, 1), (2, 7))])
+        assert torch.equal(y[::2], want[:, 0])
