@@ -239,9 +239,13 @@ struct Place {
 
 // The C ABI sees the copies of gathered tensors: whether what these write in the
 // end is also written, or read, elsewhere in the call is found here.
-bool gathered_overlap(const Tensors& grads, const Tensors& out, const Gathered& gathered) {
+bool gathered_overlap(const Tensors& grads, const Tensors& out, const Gathered& gathered, PyObject* total) {
   std::vector<Place> all;
-  all.reserve(2 * grads.size());
+  all.reserve(2 * grads.size() + 1);
+  if (total != Py_None) {
+    const at::Tensor& t = THPVariable_Unpack(total);
+    all.emplace_back(t, t.const_data_ptr(), false, true);
+  }
   for (size_t i = 0, k = 0; i < grads.size(); ++i) {
     const at::Tensor &g = grads[i], &o = out[i];
     const bool there = k < gathered.size() && gathered[k].first == i;
@@ -382,7 +386,8 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       to.push_back(back.back().second.mutable_data_ptr());
     }
   }
-  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back)) check(ILQR_ERR_OVERLAP, "clip_grad_norm");
+  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back, args[5]))
+    check(ILQR_ERR_OVERLAP, "clip_grad_norm");
   const at::Tensor norm = new_tensor({}, at::kFloat, device);
   size_t bytes = 0;
   const at::Tensor ws = workspace(n, device, &bytes);
@@ -478,7 +483,8 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       segments(flat, flat, dims[i], layout + 6 * i);
     }
   }
-  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back)) check(ILQR_ERR_OVERLAP, "clip_grad_elements");
+  if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back, Py_None))
+    check(ILQR_ERR_OVERLAP, "clip_grad_elements");
   const at::Tensor norms = new_tensor({B}, at::kFloat, device);
   check(ilqr_b200_grad_clip_elements(a.in.data(), to.data(), a.types.data(), layout, (int32_t)n, B, bound.max_norm,
                                      bound.eps, zero_nonfinite ? 1 : 0, norms.mutable_data_ptr<float>(),

@@ -58,10 +58,15 @@ void sort_spans(std::vector<Span>& s) {
   if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
 }
 
+bool any_meets(const std::vector<Span>& s, const void* p, size_t bytes) {
+  const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+  return p != nullptr && std::any_of(s.begin(), s.end(), [=](const Span& x) { return x.lo < hi && lo < x.hi; });
+}
+
 // Whether a value that the call writes is also one that it writes or reads
 // elsewhere: blocks run in no order, so only a tensor's own input may be its
 // output, whole.
-bool overlaps(const List& l) {
+bool overlaps(const List& l, const double* total, const float* norm) {
   std::vector<Span> outs, ins;  // of those that are not in place
   outs.reserve((size_t)l.n);
   for (int32_t i = 0; i < l.n; ++i) {
@@ -80,7 +85,10 @@ bool overlaps(const List& l) {
     while (k < outs.size() && outs[k].hi <= x.lo) ++k;
     if (k < outs.size() && outs[k].lo < x.hi) return true;
   }
-  return false;
+  // the first block writes the norm while others may still read
+  if (total != nullptr) ins.push_back({(uintptr_t)total, (uintptr_t)(total + 1)});
+  return any_meets(outs, total, sizeof(*total)) || any_meets(outs, norm, sizeof(*norm)) ||
+         any_meets(ins, norm, sizeof(*norm));
 }
 
 uint64_t chunks_of(int64_t numel, int32_t dtype, uint32_t chunk_bytes) {
@@ -258,7 +266,7 @@ int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_
     return status_of(join_all(s.max_type != 0, total, 1, o, stream));
   }
   try {
-    if (overlaps(l)) return ILQR_ERR_OVERLAP;
+    if (overlaps(l, total, norm)) return ILQR_ERR_OVERLAP;
     if (total == nullptr && is_small(l))
       return small_impl(l, s.max_type != 0, &s, ilqr::GradNormOut{norm, nullptr, nullptr}, stream);
     if (n_tensors <= ilqr::GRAD_CAP_SHORT) return clip_impl<ilqr::GRAD_CAP_SHORT>(l, s, total, norm, slots, stream);
@@ -381,11 +389,14 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
     row_bytes += words * 16;
     if (r.dtype != tab.t[0].dtype) tab.one_dtype = 0;
   }
-  for (int a = 0; a < tab.n; ++a)
+  const Rows all_norms{(uintptr_t)norms, 0, 0, norms != nullptr ? B * (int64_t)sizeof(float) : 0, 1, 1};
+  for (int a = 0; a < tab.n; ++a) {
+    if (!disjoint(outs[a], all_norms) || !disjoint(ins[a], all_norms)) return ILQR_ERR_OVERLAP;
     for (int b = 0; b < tab.n; ++b) {
       if (a != b && (!disjoint(outs[a], outs[b]) || !disjoint(outs[a], ins[b]))) return ILQR_ERR_OVERLAP;
       if (a == b && !same(ins[a], outs[a]) && !disjoint(outs[a], ins[a])) return ILQR_ERR_OVERLAP;
     }
+  }
   // in place is told by the address alone in the kernel
   tab.B = B;
   tab.max_norm = max_norm;

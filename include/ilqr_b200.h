@@ -506,7 +506,8 @@ int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const in
  * out = c grads over a list, c = min(1, max_norm / (norm + eps)); max_norm =
  * infinity leaves the values as they are, a NaN norm makes them NaN. out: HOST
  * array of device pointers; out[i] may be grads[i] (in place), otherwise no
- * output may share memory with any other tensor of the call (ILQR_ERR_OVERLAP).
+ * output, norm among them, may share memory with any other tensor of the call,
+ * total among them (ILQR_ERR_OVERLAP).
  * total: device, the sum of squares (largest magnitude) to clip by, or NULL
  * for the list's own. norm (device, NULL to skip): the norm before clipping.
  */

@@ -122,3 +122,18 @@ def test_in_place_through_another_view():
         want = form([y.as_strided((10, 1), (2, 1))], 0.1)[0][0]
         form([y.as_strided((10, 1), (2, 1))], 0.1, out=[y.as_strided((10, 1), (2, 7))])
         assert torch.equal(y[::2], want[:, 0])
+
+
+def test_a_total_within_an_output_is_refused():
+    g = _values((400,), F32, 1)
+    y = torch.zeros(800, device=DEV)
+    total = y.view(torch.float64)[30]                # values 60 and 61
+    total.copy_(nat.grad_norm_total([g]))
+    _refused(lambda: nat.clip_grad_norm([g], 0.5, total=total, out=[y[:400]]), y)
+    _refused(lambda: nat.clip_grad_norm([g], 0.5, total=total, out=[y[::2]]), y)
+    got, n = nat.clip_grad_norm([g], 0.5, total=total, out=[y[62:462]])
+    want, m = nat.clip_grad_norm([g], 0.5, total=total.clone(), out=[torch.zeros(800, device=DEV)[62:462]])
+    assert torch.equal(n, m) and torch.equal(got[0], want[0])
+    # one that is part of a gradient that is only read
+    both, n = nat.clip_grad_norm([y[60:62]], 0.5, total=total)
+    assert torch.equal(n, m)

@@ -11,6 +11,7 @@ import subprocess
 import pytest
 import torch
 
+import ilqr_native as nat
 from test_gradclip_host import A, _elements
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -118,3 +119,37 @@ def test_columns_of_one_array_are_taken(T, B, time_major):
     lay = ((1, 10, 0, R, 0, R), (T, 196, 210, R, 210, R), (T, 14, 210, R, 210, R))
     at = (A, A + 40, A + 40 + 784)
     assert _elements(grads=at, out=at, dtypes=(0, 0, 0), layout=lay, B=B) == 4
+
+
+# ---- what a call writes or reads beside the gradients ----------------------------
+
+def _raw_clip(total=None, norm=None, grads=(A, 2 * A), out=(3 * A, 4 * A), numel=(50, 70)):
+    arr = [(ctypes.c_uint64 * 2)(*grads), (ctypes.c_uint64 * 2)(*out), (ctypes.c_int64 * 2)(*numel), (ctypes.c_int32 * 2)(0, 0)]
+    return nat.lib().ilqr_b200_grad_clip(*arr, 2, 0, 1.0, 1e-6, total, norm, 8 * A, 1 << 20, None)
+
+
+def _raw_elements(norms, in_place=True, B=16, T=5):
+    arr = [(ctypes.c_uint64 * 1)(A), (ctypes.c_uint64 * 1)(A if in_place else 4 * A), (ctypes.c_int32 * 1)(0),
+           (ctypes.c_int64 * 6)(T, 14, 210, 210 * T, 210, 210 * T)]
+    return nat.lib().ilqr_b200_grad_clip_elements(*arr, 1, B, 1.0, 1e-6, 0, norms, None)
+
+
+def test_total_and_norm_that_share_memory_are_refused():
+    assert _raw_clip(total=3 * A) == 7 and _raw_clip(total=4 * A + 272) == 7       # within an output, at its end
+    assert _raw_clip(total=A, out=(A, 4 * A)) == 7                                 # and in place
+    assert _raw_clip(norm=3 * A + 196) == 7 and _raw_clip(norm=A + 196) == 7       # an output, an input
+    assert _raw_clip(total=6 * A, norm=6 * A) == 7 and _raw_clip(total=6 * A, norm=6 * A + 4) == 7
+    for in_place in (True, False):
+        assert _raw_elements(A, in_place) == 7                                     # over the first element
+        assert _raw_elements(A + 4 * (210 * 79 + 13), in_place) == 7               # from the last value on
+        assert _raw_elements(A + 780, in_place) == 7                               # from a gap into the next run
+    assert _raw_elements(4 * A, False) == 7
+
+
+@no_gpu
+def test_total_and_norm_beside_the_tensors_are_taken():
+    assert _raw_clip(total=3 * A + 200, norm=3 * A + 208) == 4                     # behind an output
+    assert _raw_clip(total=A) == 4                                                 # an input that is only read
+    for in_place in (True, False):
+        assert _raw_elements(A + 4 * (210 * 79 + 14), in_place) == 4
+        assert _raw_elements(A + 776, in_place) == 4                               # within a gap
