@@ -20,6 +20,8 @@ using ilqr::GradTable;
 
 int status_of(cudaError_t e) { return e == cudaSuccess ? ILQR_OK : ILQR_ERR_CUDA; }
 
+bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
 int64_t size_of(int32_t dtype) { return dtype == ILQR_DTYPE_F32 ? 4 : 2; }
 
 constexpr int64_t MAX_VALUES = (int64_t)1 << 40;  // of a list: chunk numbers stay in 32 bits
@@ -226,6 +228,8 @@ int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const in
   const List l{grads, nullptr, numel, dtypes, n_tensors};
   if (const int st = check_list(l, norm_type); st != ILQR_OK) return st;
   if (norm == nullptr && tensor_norms == nullptr && total == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
+  if (!aligned(norm, sizeof(float)) || !aligned(tensor_norms, sizeof(float)) || !aligned(total, sizeof(double)))
+    return ILQR_ERR_MISALIGNED;
   if (n_tensors == 0) {
     cudaError_t e = cudaSuccess;
     if (norm != nullptr) e = cudaMemsetAsync(norm, 0, sizeof(float), stream);
@@ -233,7 +237,7 @@ int ilqr_b200_grad_norm(const void* const* grads, const int64_t* numel, const in
     return status_of(e);
   }
   if (workspace == nullptr || workspace_bytes < slots_of(n_tensors) * sizeof(double)) return ILQR_ERR_WORKSPACE;
-  if ((uintptr_t)workspace & 7u) return ILQR_ERR_MISALIGNED;
+  if (!aligned(workspace, sizeof(double))) return ILQR_ERR_MISALIGNED;
   try {
     const ilqr::GradNormOut o{norm, tensor_norms, total};
     double* slots = static_cast<double*>(workspace);
@@ -254,9 +258,9 @@ int ilqr_b200_grad_clip(const void* const* grads, void* const* out, const int64_
   const List l{grads, out, numel, dtypes, n_tensors};
   if (const int st = check_list(l, norm_type); st != ILQR_OK) return st;
   if (!(max_norm >= 0.0) || !(eps >= 0.0) || std::isinf(eps)) return ILQR_ERR_INVALID_ARGUMENT;
-  if (total != nullptr && ((uintptr_t)total & 7u)) return ILQR_ERR_MISALIGNED;
+  if (!aligned(total, sizeof(double)) || !aligned(norm, sizeof(float))) return ILQR_ERR_MISALIGNED;
   if (workspace == nullptr || workspace_bytes < slots_of(n_tensors) * sizeof(double)) return ILQR_ERR_WORKSPACE;
-  if ((uintptr_t)workspace & 7u) return ILQR_ERR_MISALIGNED;
+  if (!aligned(workspace, sizeof(double))) return ILQR_ERR_MISALIGNED;
   double* slots = static_cast<double*>(workspace);
   const ilqr::GradScale s{max_norm, eps, norm_type == ILQR_NORM_MAX ? 1 : 0};
   if (n_tensors == 0) {
@@ -330,6 +334,7 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
     return ILQR_ERR_INVALID_ARGUMENT;
   if (grads == nullptr || out == nullptr || dtypes == nullptr || layout == nullptr) return ILQR_ERR_INVALID_ARGUMENT;
   if (!(max_norm >= 0.0) || !(eps >= 0.0) || std::isinf(eps)) return ILQR_ERR_INVALID_ARGUMENT;
+  if (!aligned(norms, sizeof(float))) return ILQR_ERR_MISALIGNED;
   if (B == 0) return ILQR_OK;
   constexpr int64_t FAR = (int64_t)1 << 44;  // bytes: no address arithmetic below can wrap
   ilqr::RowTable tab;
