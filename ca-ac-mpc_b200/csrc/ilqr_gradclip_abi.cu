@@ -210,7 +210,7 @@ int small_impl(const List& l, bool max_type, const ilqr::GradScale* s, const ilq
   return status_of(ilqr::launch_grad_small(tab, max_type, s, o, stream));
 }
 
-int64_t magnitude(int64_t v) { return v < 0 ? -v : v; }
+uint64_t magnitude(int64_t v) { return v < 0 ? 0 - (uint64_t)v : (uint64_t)v; }
 
 }  // namespace
 
@@ -352,7 +352,7 @@ int ilqr_b200_grad_clip_elements(const void* const* grads, void* const* out, con
     if (n_seg > INT32_MAX || len > INT32_MAX || n_seg * len > INT32_MAX) return ILQR_ERR_INVALID_ARGUMENT;
     for (int k = 2; k < 6; ++k) {
       const int64_t times = (k & 1) ? B : n_seg;  // [2] in_seg, [3] in_row, [4] out_seg, [5] out_row
-      if (magnitude(g[k]) > FAR / sz || (times > 1 && magnitude(g[k]) > FAR / sz / times))
+      if (magnitude(g[k]) > (uint64_t)(FAR / sz / std::max<int64_t>(times, 1)))
         return ILQR_ERR_INVALID_ARGUMENT;
     }
     if (grads[i] == nullptr || out[i] == nullptr) return ILQR_ERR_INVALID_ARGUMENT;

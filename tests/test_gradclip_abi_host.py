@@ -39,3 +39,14 @@ def test_misaligned_totals_are_refused(off):
         assert _norm(norm=None, total=A + off, n=n) == 2
     for n in (0, 1):
         assert _clip(total=4 * A + off, n=n) == 2
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("k", [2, 3, 4, 5])
+def test_the_lowest_stride_is_refused(k, dtype):
+    """-2^63, whose magnitude is no 64-bit integer; its bytes wrap to stride 0."""
+    for lowest in (-2**63, -2**63 + 1, 2**63 - 1, -2**62):
+        layout = [2, 10, 10, 20, 10, 20]
+        layout[k] = lowest
+        assert _elements(layout, dtype=dtype) == 1
+        assert _elements([1, *layout[1:]], dtype=dtype, B=1) == 1
