@@ -106,6 +106,12 @@ double number(PyObject* o) {
   return v;
 }
 
+int64_t dimension(PyObject* o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
 int32_t norm_code(PyObject* norm_type) {
   const double p = number(norm_type);
   TORCH_CHECK_VALUE(p == 2.0 || p == INFINITY, "norm_type must be 2 or inf, not ", p);
@@ -442,19 +448,20 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   const bool each = !PyLong_Check(args[2]);
   const Object given_out(given_outputs(args[1]));
   const Object given_dims(each ? PySequence_List(args[2]) : Py_NewRef(args[2]));
+  c10::SmallVector<int64_t, ILQR_MAX_ELEMENT_TENSORS> dims;
+  for (Py_ssize_t i = 0, k = each ? PyList_GET_SIZE(given_dims.p) : 1; i < k; ++i)
+    dims.push_back(dimension(each ? PyList_GET_ITEM(given_dims.p, i) : given_dims.p));
   const Object given(as_list(args[0], "grads"));
+  // all that may run the caller's code has come before the first tensor is read
   Tensors grads, out;
   read_list(given.p, grads);
   const size_t n = grads.size();
   TORCH_CHECK(n >= 1 && n <= ILQR_MAX_ELEMENT_TENSORS, "grads must hold 1 to ", ILQR_MAX_ELEMENT_TENSORS,
               " tensors, got ", n);
-  int64_t dims[ILQR_MAX_ELEMENT_TENSORS];
-  TORCH_CHECK(!each || (size_t)PyList_GET_SIZE(given_dims.p) == n, "batch_dims must hold ", n, " numbers, got ",
-              each ? PyList_GET_SIZE(given_dims.p) : 0);
+  TORCH_CHECK(!each || dims.size() == n, "batch_dims must hold ", n, " numbers, got ", dims.size());
+  if (!each) dims.assign(n, dims[0]);
   int64_t B = 0;
   for (size_t i = 0; i < n; ++i) {
-    dims[i] = PyLong_AsLongLong(each ? PyList_GET_ITEM(given_dims.p, i) : given_dims.p);
-    if (dims[i] == -1 && PyErr_Occurred()) throw python_error();
     TORCH_CHECK(dims[i] >= 0 && dims[i] < grads[i].dim(), "batch dimension ", dims[i], " of a tensor of shape ",
                 grads[i].sizes());
     if (i == 0) B = grads[0].size(dims[0]);
