@@ -445,7 +445,8 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   TORCH_CHECK_TYPE(nargs == 6, "clip_grad_elements takes six values");
   const Bound bound(args[3], args[4]);
   const bool zero_nonfinite = truth(args[5]);
-  const bool each = !PyLong_Check(args[2]);
+  // a number of any kind (NumPy's among them); tensors and arrays count as sequences
+  const bool each = !PyIndex_Check(args[2]) || Py_TYPE(args[2])->tp_iter != nullptr;
   const Object given_out(given_outputs(args[1]));
   const Object given_dims(each ? PySequence_List(args[2]) : Py_NewRef(args[2]));
   c10::SmallVector<int64_t, ILQR_MAX_ELEMENT_TENSORS> dims;
