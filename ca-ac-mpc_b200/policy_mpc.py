@@ -111,6 +111,7 @@ class PolicyMPC:
         return torch.cat((thrust_normalized.unsqueeze(1), omegas_normalized), dim=1)
 
 
+@torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> Tensor:
     """Clip the gradients of the policy's parameters in place by their norm
