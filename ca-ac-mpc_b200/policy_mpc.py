@@ -112,16 +112,18 @@ class PolicyMPC:
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> Tensor:
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
+                    norm_type: Union[float, str] = 2.0, error_if_nonfinite: bool = False) -> Tensor:
     """Clip the gradients of the policy's parameters in place by their norm
     together, as the update does between its backward and the optimiser's step
     (th.nn.utils.clip_grad_norm_(policy.parameters(), max_grad_norm),
     stable_baselines3/ppo/ppo.py:274-277): its arguments (but foreach) and its
     result, the norm before clipping as a device scalar. Parameters without a gradient are
     passed over; parameters on several devices are clipped by their joint
-    norm. norm_type: 2 or inf. Nothing reads back to the host unless
+    norm. norm_type: 2 or inf (or "inf"). A gradient that two of them share is
+    refused: it would be scaled twice. Nothing reads back to the host unless
     error_if_nonfinite asks for it."""
+    norm_type = float(norm_type)
     params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
@@ -133,7 +135,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     if len(lists) > 1 or error_if_nonfinite:
         first = grads[0].device
         each = torch.stack([_nat.grad_norm_total(held, norm_type).to(first) for held in lists.values()])
-        total = each.sum() if float(norm_type) == 2.0 else each.max()
+        total = each.sum() if norm_type == 2.0 else each.max()
         if error_if_nonfinite and not torch.isfinite(total):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, "
                                "so it cannot be clipped.")

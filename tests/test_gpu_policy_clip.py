@@ -28,3 +28,12 @@ def test_gradients_with_history_are_clipped_as_torch_clips_them():
             w.grad = None
         assert abs(pair[0][1] - pair[1][1]) <= 2.0**-18 * pair[0][1]
         assert torch.allclose(pair[0][0], pair[1][0], rtol=2.0**-18, atol=0.0)
+
+
+def test_norm_type_as_text():
+    w = torch.zeros(3, device=DEV, requires_grad=True)
+    w.grad = torch.tensor([3.0, 0.0, -4.0], device=DEV)
+    assert float(policy_mpc.clip_grad_norm_([w], 2.0, norm_type="inf", error_if_nonfinite=True)) == 4.0
+    assert torch.allclose(w.grad, torch.tensor([1.5, 0.0, -2.0], device=DEV), rtol=1e-6)
+    with pytest.raises(ValueError, match="norm_type"):
+        policy_mpc.clip_grad_norm_([w], 1.0, norm_type="1")

@@ -65,3 +65,16 @@ def test_gradients_with_history_are_clipped(plain):
     n = policy_mpc.clip_grad_norm_([w], 0.5)
     assert torch.is_grad_enabled() and not n.requires_grad and w.grad._version > version
     assert torch.allclose(w.grad.detach(), before * 0.5 / (before.norm() + 1e-6))
+
+
+def test_norm_types_that_torch_takes(plain):
+    for given, want in (("inf", math.inf), (math.inf, math.inf), ("2", 2.0), (2, 2.0), (torch.tensor(2.0), 2.0)):
+        a, b = _net(), _net()
+        bound = 0.3 * float(torch.nn.utils.get_total_norm([q.grad for q in a.parameters()], want))
+        na = torch.nn.utils.clip_grad_norm_(a.parameters(), bound, norm_type=given)
+        nb = policy_mpc.clip_grad_norm_(b.parameters(), bound, norm_type=given)
+        assert math.isclose(float(na), float(nb), rel_tol=2.0**-18)
+        for u, v in zip(a.parameters(), b.parameters()):
+            assert torch.allclose(u.grad, v.grad, rtol=2.0**-18, atol=0.0)
+    with pytest.raises(ValueError):
+        policy_mpc.clip_grad_norm_(_net().parameters(), 1.0, norm_type="two")
