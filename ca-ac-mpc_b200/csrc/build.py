@@ -8,7 +8,9 @@ arithmetic rounds like the reference's elementwise torch ops; FILE_FLAGS adds
 per-file options) and links them
 into ca-ac-mpc_b200/libilqr_b200.so, then the torch binding of the calls that
 take lists of tensors (binding/ilqr_torch.cpp) with g++ into
-ca-ac-mpc_b200/ilqr_torch.so, a Python module. Objects are rebuilt only when a
+ca-ac-mpc_b200/ilqr_torch.so, a Python module. The library needs no torch: where
+what the binding is built with is not there, it is left out with a message, and
+its calls say so. Objects are rebuilt only when a
 source or header is newer than the object (make-style), in parallel.
 """
 
@@ -18,6 +20,7 @@ import argparse
 import concurrent.futures as cf
 import glob
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -30,8 +33,10 @@ LIB = os.path.join(PKG, "libilqr_b200.so")
 PROBE_LIB = os.path.join(PKG, "libilqr_probe.so")
 PROBE_SRC = os.path.join(HERE, "probe", "fma_probe.cu")
 BINDING_SRC = os.path.join(HERE, "binding", "ilqr_torch.cpp")
+BINDING_FILES = [BINDING_SRC, os.path.join(ROOT, "include", "ilqr_b200.h"), os.path.join(HERE, "ilqr_overlap.h")]
 BINDING = os.path.join(PKG, "ilqr_torch.so")
 NVCC = os.environ.get("NVCC", "nvcc")
+CXX = "g++"  # as nvcc takes it (torch and the binding share one libstdc++)
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-fmad=false", "-Xcompiler", "-fPIC,-O2",
          "-I", os.path.join(ROOT, "include"), "-I", HERE]
@@ -49,21 +54,42 @@ def _newer(src_files, target):
     return any(os.path.getmtime(s) > t for s in src_files)
 
 
+def binding_needs() -> list:
+    """What the torch binding is built with and is not here."""
+    if shutil.which(CXX) is None:
+        return [CXX]
+    try:
+        import torch
+    except ImportError:
+        return ["torch"]
+    at = os.path.dirname(torch.__file__)
+    files = [os.path.join(at, "include", "torch", "csrc", "autograd", "python_variable.h"),
+             os.path.join(at, "include", "c10", "cuda", "CUDAGuard.h"),
+             os.path.join(_cuda_home(), "include", "cuda_runtime_api.h"),
+             os.path.join(sysconfig.get_paths()["include"], "Python.h"),
+             *(os.path.join(at, "lib", f"lib{n}.so") for n in TORCH_LIBS)]
+    return [f for f in files if not os.path.exists(f)]
+
+
+def _cuda_home() -> str:
+    return os.environ.get("CUDA_HOME", "/usr/local/cuda")
+
+
+TORCH_LIBS = ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")
+
+
 def build_binding() -> str:
     """The torch binding, against the torch that is importable here and the
     C-ABI library beside it."""
     import torch
     at = os.path.dirname(torch.__file__)
-    headers = [os.path.join(ROOT, "include", "ilqr_b200.h"), os.path.join(HERE, "ilqr_overlap.h")]
-    # g++ as nvcc takes it (torch and this module share one libstdc++)
-    if _newer([BINDING_SRC, *headers, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
+    if _newer([*BINDING_FILES, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
         inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
-               os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
-               sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
-        cmd = ["g++", "-std=c++20", "-O2", "-fPIC", "-shared",
+               os.path.join(_cuda_home(), "include"), sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+        cmd = [CXX, "-std=c++20", "-O2", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc],
-               BINDING_SRC, "-o", BINDING, f"-L{os.path.join(at, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-               "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{PKG}", "-l:libilqr_b200.so", "-Wl,-rpath,$ORIGIN"]
+               BINDING_SRC, "-o", BINDING, f"-L{os.path.join(at, 'lib')}", *[f"-l{n}" for n in TORCH_LIBS],
+               f"-L{PKG}", "-l:libilqr_b200.so", "-Wl,-rpath,$ORIGIN"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("torch binding build failed:\n" + r.stdout + r.stderr)
@@ -106,7 +132,6 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(link, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
-    build_binding()
     # FP32 FMA throughput probe used by the benchmark's roofline (separate
     # library: measurement only).
     if _newer([PROBE_SRC], PROBE_LIB):
@@ -114,6 +139,14 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("probe build failed:\n" + r.stdout + r.stderr)
+    missing = binding_needs()
+    if missing:
+        if os.path.exists(BINDING) and _newer(BINDING_FILES, BINDING):
+            os.remove(BINDING)  # of an earlier source
+        print("the torch binding of the gradient norms and clipping was not built, for want of: " + ", ".join(missing),
+              file=sys.stderr)
+    else:
+        build_binding()
     return LIB
 
 
