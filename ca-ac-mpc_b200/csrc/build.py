@@ -11,7 +11,8 @@ take lists of tensors (binding/ilqr_torch.cpp) with g++ into
 ca-ac-mpc_b200/ilqr_torch.so, a Python module. The library needs no torch: where
 what the binding is built with is not there, it is left out with a message, and
 its calls say so. Objects are rebuilt only when a
-source or header is newer than the object (make-style), in parallel.
+source or header is newer than the object (make-style), in parallel, the binding
+also when torch or Python is another than it was built with.
 """
 
 from __future__ import annotations
@@ -83,16 +84,24 @@ def build_binding() -> str:
     C-ABI library beside it."""
     import torch
     at = os.path.dirname(torch.__file__)
-    if _newer([*BINDING_FILES, os.path.join(at, "version.py"), os.path.abspath(__file__)], BINDING):
-        inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
-               os.path.join(_cuda_home(), "include"), sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
-        cmd = [CXX, "-std=c++20", "-O2", "-fPIC", "-shared",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc],
-               BINDING_SRC, "-o", BINDING, f"-L{os.path.join(at, 'lib')}", *[f"-l{n}" for n in TORCH_LIBS],
-               f"-L{PKG}", "-l:libilqr_b200.so", "-Wl,-rpath,$ORIGIN"]
+    inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           os.path.join(_cuda_home(), "include"), sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+    cmd = [CXX, "-std=c++20", "-O2", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc],
+           BINDING_SRC, "-o", BINDING, f"-L{os.path.join(at, 'lib')}", *[f"-l{n}" for n in TORCH_LIBS],
+           f"-L{PKG}", "-l:libilqr_b200.so", "-Wl,-rpath,$ORIGIN"]
+    # what it was built against: files of another torch may be older than it
+    made = "\n".join([torch.__version__, str(torch.version.git_version), sys.version, *cmd])
+    stamp = os.path.join(OBJ_DIR, "ilqr_torch.stamp")
+    if _newer(BINDING_FILES, BINDING) or not os.path.exists(stamp) or open(stamp).read() != made:
+        os.makedirs(OBJ_DIR, exist_ok=True)
+        if os.path.exists(stamp):
+            os.remove(stamp)  # a build that is interrupted leaves none
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("torch binding build failed:\n" + r.stdout + r.stderr)
+        with open(stamp, "w") as f:
+            f.write(made)
     return BINDING
 
 

@@ -73,3 +73,35 @@ def test_a_binding_that_does_not_compile_is_an_error_after_the_rest(build, monke
     with pytest.raises(RuntimeError, match="binding"):
         build.build()
     assert os.path.exists(build.LIB) and os.path.exists(build.PROBE_LIB)
+
+
+def test_another_torch_or_python_rebuilds_the_binding(build, monkeypatch):
+    """Also one whose files are older than the binding."""
+    import torch
+    build.build()
+    _ran(build)
+    for owner, name, value in ((torch, "__version__", "9.9.9"), (torch.version, "git_version", "0" * 40),
+                               (build.sys, "version", "3.99")):
+        with monkeypatch.context() as m:
+            m.setattr(owner, name, value)
+            build.build()
+            assert _ran(build) == ["binding"], name
+            build.build()
+            assert _ran(build) == [], name
+        build.build()
+        assert _ran(build) == ["binding"], name
+    os.utime(build.BINDING, (1, 1))
+    build.build()
+    assert _ran(build) == ["binding"]
+
+
+def test_a_binding_that_failed_is_tried_again(build, monkeypatch):
+    build.build()
+    os.utime(build.BINDING, (1, 1))
+    with monkeypatch.context() as m:
+        m.setattr(build, "CXX", "/bin/false")
+        with pytest.raises(RuntimeError, match="binding"):
+            build.build()
+    _ran(build)
+    build.build()
+    assert _ran(build) == ["binding"]
