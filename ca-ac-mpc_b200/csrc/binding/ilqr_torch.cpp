@@ -230,7 +230,7 @@ struct Place {
     step = dims[0].stride;
     at = (int64_t)(lo % (uintptr_t)step);
   }
-  // Columns of one array, the usual case, without a search.
+  // Columns of one array, without a search.
   bool beside(const Place& x) const {
     return step > 0 && step == x.step && at + len <= step && x.at + x.len <= step &&
            (at + len <= x.at || x.at + x.len <= at);
@@ -242,6 +242,21 @@ struct Place {
                       [](const ilqr::Every& a, const ilqr::Every& b) { return a.count == b.count && a.stride == b.stride; });
   }
 };
+
+// Whether all of them are columns of one array that end before the next begins.
+bool all_beside(const std::vector<Place>& all) {
+  std::vector<std::pair<int64_t, int64_t>> c;
+  c.reserve(all.size() + 1);
+  for (const Place& p : all) {
+    if (p.step == 0 || p.step != all[0].step) return false;
+    c.emplace_back(p.at, p.at + p.len);
+  }
+  std::sort(c.begin(), c.end());
+  c.emplace_back(all[0].step, 0);
+  for (size_t k = 1; k < c.size(); ++k)
+    if (c[k - 1].second > c[k].first) return false;
+  return true;
+}
 
 // The C ABI sees the copies of gathered tensors: whether what these write in the
 // end is also written, or read, elsewhere in the call is found here.
@@ -261,6 +276,7 @@ bool gathered_overlap(const Tensors& grads, const Tensors& out, const Gathered& 
     Place in(g, g.const_data_ptr(), false, there);
     if (!in.is(all.back())) all.push_back(std::move(in));
   }
+  if (all.empty() || all_beside(all)) return false;
   std::sort(all.begin(), all.end(), [](const Place& a, const Place& b) { return a.lo < b.lo; });
   for (size_t a = 0; a < all.size(); ++a)
     for (size_t b = a + 1; b < all.size() && all[b].lo < all[a].hi; ++b)

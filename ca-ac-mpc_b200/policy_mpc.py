@@ -111,7 +111,6 @@ class PolicyMPC:
         return torch.cat((thrust_normalized.unsqueeze(1), omegas_normalized), dim=1)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
                     norm_type: Union[float, str] = 2.0, error_if_nonfinite: bool = False) -> Tensor:
     """Clip the gradients of the policy's parameters in place by their norm
@@ -123,7 +122,15 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     norm. norm_type: 2 or inf (or "inf"). A gradient that two of them share is
     refused: it would be scaled twice. Nothing reads back to the host unless
     error_if_nonfinite asks for it."""
-    norm_type = float(norm_type)
+    enabled = torch.is_grad_enabled()
+    torch._C._set_grad_enabled(False)  # what torch.no_grad() does, for a microsecond of host time less
+    try:
+        return _clip_grad_norm(parameters, max_norm, float(norm_type), error_if_nonfinite)
+    finally:
+        torch._C._set_grad_enabled(enabled)
+
+
+def _clip_grad_norm(parameters, max_norm, norm_type, error_if_nonfinite):
     params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:

@@ -157,3 +157,15 @@ def test_a_norm_that_is_not_finite_is_reported_before_anything_is_written(plain,
         policy_mpc.clip_grad_norm_(params, 0.5, norm_type=p, error_if_nonfinite=True)
     assert all(torch.equal(g.as_subclass(torch.Tensor).nan_to_num(7.0), b.nan_to_num(7.0)) for g, b in zip(grads, before))
     assert not any(kind == "clip" for kind, _ in plain.calls)
+
+
+def test_grad_mode_is_left_as_it_was(plain):
+    for enabled in (True, False):
+        with torch.set_grad_enabled(enabled):
+            w = torch.nn.Parameter(torch.ones(3))
+            w.grad = torch.ones(3)
+            policy_mpc.clip_grad_norm_([w], 1.0)
+            assert torch.is_grad_enabled() == enabled
+            with pytest.raises(ValueError):
+                policy_mpc.clip_grad_norm_([], 1.0, norm_type="two")
+            assert torch.is_grad_enabled() == enabled
