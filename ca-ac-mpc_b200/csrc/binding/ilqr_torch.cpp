@@ -492,11 +492,12 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   at::NoGradGuard no_grad;
   Arrays a;
   Small<void*> to;
-  int64_t layout[6 * ILQR_MAX_ELEMENT_TENSORS];
+  int64_t layout[6 * ILQR_MAX_ELEMENT_TENSORS] = {};
   Gathered back;
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor &g = grads[i], &o = out[i];
-    if (!g.is_neg() && !o.is_neg() && segments(g, o, dims[i], layout + 6 * i)) {
+    // a tensor without values has no segments
+    if (g.numel() == 0 || (!g.is_neg() && !o.is_neg() && segments(g, o, dims[i], layout + 6 * i))) {
       a.add(g);
       to.push_back(o.mutable_data_ptr());
     } else {
@@ -504,7 +505,7 @@ PyObject* clip_grad_elements(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       const at::Tensor& flat = back.back().second;
       a.add(flat);
       to.push_back(flat.mutable_data_ptr());
-      segments(flat, flat, dims[i], layout + 6 * i);
+      TORCH_INTERNAL_ASSERT(segments(flat, flat, dims[i], layout + 6 * i));
     }
   }
   if (!back.empty() && args[1] != Py_None && gathered_overlap(grads, out, back, Py_None))

@@ -137,3 +137,24 @@ def test_a_total_within_an_output_is_refused():
     # one that is part of a gradient that is only read
     both, n = nat.clip_grad_norm([y[60:62]], 0.5, total=total)
     assert torch.equal(n, m)
+
+
+def test_empty_tensors_of_every_shape():
+    """An element has no values in them, whatever their strides and batch dimension."""
+    import itertools
+    full = [_values((4, 6, 8), F32, k)[..., 1:] for k in range(8)]
+    for shape in itertools.product((0, 1, 3), repeat=4):
+        if 0 not in shape:
+            continue
+        wide = torch.zeros([2 * s + 1 for s in shape], device=DEV)
+        gaps = wide[tuple(slice(0, 2 * s, 2) for s in shape)]
+        assert gaps.shape == shape
+        for dim, B in enumerate(shape):
+            x = _values((B, 7), F32, dim)
+            for empty in (torch.zeros(shape, device=DEV), gaps, gaps.permute(3, 1, 0, 2).contiguous().permute(2, 1, 3, 0)):
+                for out in (None, [empty, x]):
+                    # right after a call whose layouts have values everywhere
+                    nat.clip_grad_elements(full, 1.0, out=full)
+                    _, n = nat.clip_grad_elements([empty], 1.0, batch_dims=dim, out=out and [empty])
+                    assert n.tolist() == [0.0] * B
+                    _check_elements([empty, x], [dim, 0], 1.5, out=out)
