@@ -3,7 +3,7 @@
 // These calls take lists of up to thousands of tensors, whose addresses, sizes,
 // types and strides are read here: the same reading through the Python
 // interface costs 0.6 us a tensor and takes longer than the kernels for most
-// lists (400 bf16 tensors of 600 MB: 246 us against 113 us of GPU time). The
+// lists (400 bf16 tensors of 600 MB: 246 us against 95 us of GPU time). The
 // calls are documented in ilqr_native.py; everything but the reading goes through
 // the C ABI in include/ilqr_b200.h.
 #include <torch/csrc/Exceptions.h>

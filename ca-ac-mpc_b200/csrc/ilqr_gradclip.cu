@@ -446,7 +446,10 @@ __device__ __forceinline__ void entry_sum(Acc<MAX>& a, uint32_t dtype, const voi
 }
 
 // Value by value: for coefficients below the floats' range, and for `in` and
-// `out` that lie differently in their 16-byte words.
+// `out` that lie differently in their 16-byte words (new outputs of views packed
+// at odd offsets). A thread has one load in flight: 200 MB of bf16 in 200 such
+// views 231 us where the vectors take 99 (both passes), 200 MB of f32 147 and 99.
+// The scaling alone runs at 21 % of DRAM's rate, its warps waiting for that load.
 __device__ __forceinline__ void entry_scale_apart(uint32_t dtype, const char* p, char* q, int64_t n, const Coef& c) {
   const int sz = dtype == ILQR_DTYPE_F32 ? 4 : 2;
 #pragma unroll 1
@@ -600,8 +603,9 @@ __device__ __forceinline__ void chunks_scale(const GradTable<CAP>& tab, uint32_t
 
 // A wave of blocks with a run of chunks each; every block joins the partial sums
 // for itself, in the same order, instead of a launch between the two. For lists
-// that L2 holds: 24 MB 15.7 us out of place with the sums; 32 MB below the bound
-// and in place 8.5 us.
+// that L2 holds: 20 MB of bf16 16.1 us out of place with the sums; 32 MB below
+// the bound and in place 9.4 us. Four blocks on an SM leave a thread 64 registers,
+// of which the vectors in flight take most: 40 bytes of the rest are spilled.
 template <int CAP>
 __global__ void __launch_bounds__(BLK, 4) grad_scale_kernel(const __grid_constant__ GradTable<CAP> tab, GradScale s,
                                                             const double* slots, int64_t n_slots, float* norm) {
@@ -983,12 +987,17 @@ __device__ __forceinline__ RowTensor part_of(const RowTensor& r, uint32_t rank, 
 // G threads for each element, whose slices are staged in shared memory: global
 // memory is read once and written once. CLUSTER: the blocks of a cluster share
 // one element. Bound by DRAM for elements of some KB and more: B = 65536, T = 50
-// time-major 869 us for 5.5 GB (6.34 TB/s, 97 % of the copy rate); B = 16384,
-// T = 20 95 us time-major, 86 us batch-major for 552 MB; the 13-state model,
+// time-major 878 us for 5.5 GB (6.28 TB/s, 96 % of the copy rate); B = 16384,
+// T = 20 94 us time-major, 87 us batch-major for 552 MB; the 13-state model,
 // B = 4096, T = 20 33 us for 201 MB. What the time-major layout costs it costs in
 // writing (reading alone 112 us against 109, T = 50, 0.8 GB; with writing 250
-// against 230), and the more the more segments an element has. Shorter elements
-// are bound by instructions: B = 16384 sigmoid rows of 2.3 KB 14.7 us for 75 MB.
+// against 230), and the more the more segments an element has. Segments of 16-bit
+// values that are no whole 16-byte words (392 bytes, and 28) cost instructions
+// besides: 2490 of a warp for each element of 8.4 KB, issued in 55 % of the
+// cycles, 70 us for 276 MB. Shorter elements are bound by instructions and by the
+// wait of a warp for its few loads: B = 16384 sigmoid rows of 2.3 KB 15 us for
+// 75 MB; B = 65536 rows of 300 bytes of bf16 1290 instructions for a warp's eight,
+// 16.6 us for 39 MB (of 600 bytes of f32 1000, 18.5 us for 79 MB).
 template <int G, int THREADS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
     grad_rows_kernel(const __grid_constant__ RowTable tab) {
@@ -1109,7 +1118,7 @@ __global__ void __launch_bounds__(THREADS, G <= 32 ? 1280 / THREADS : 1)
 
 // Elements that the shared memory of a cluster cannot hold: its blocks share one,
 // and both passes read global memory. 64 elements of 2.8 MB 100 us, 300 of 2 MB
-// 312 us (3.9 TB/s of what must move); a single one of 52 MB 248 us, what eight SMs
+// 310 us (3.9 TB/s of what must move); a single one of 52 MB 248 us, what eight SMs
 // can read and write.
 __global__ void __launch_bounds__(LONG_BLK) grad_long_rows_kernel(const __grid_constant__ RowTable tab) {
   __shared__ double sh[33];
@@ -1296,33 +1305,34 @@ cudaError_t launch_grad_rows(const RowTable& tab, cudaStream_t stream) {
   // Threads for an element by what it stages. More threads cost instructions
   // that every element repeats (its records, the join, square root and quotient),
   // fewer leave the additions of long elements to few: us by threads, bytes of an
-  // element and number of elements (without the pairs below):
+  // element of float32 and number of elements (without the pairs below):
   //     bytes (elements)    4     8    16    32    64   128   256
-  //       266 (100000)     15    19    31    55   120   205
-  //       602  (60000)     16    18    25    40    82   141
-  //      1722  (40000)     30    25    28    39    75   129
-  //      2282  (65536)     53    49    48    52    93   161
-  //      4242  (16384)     40    36    28    27    39    60
-  //      8442  (16384)    117    82    58    49    49    70   129
-  //     16842  (16384)                 113    86    86    86   121
-  //     24534   (4096)                  93    64    52    49    56
-  //     42042  (65536)                      1409   877   887   873
-  //     84042   (2048)                              92    76    72
-  //    210042   (1024)                             157   119   111
+  //       264 (100000)     15    19    31    55   120   205
+  //       600  (60000)     16    18    25    40    82   141
+  //      1720  (40000)     30    25    28    39    75   129
+  //      2280  (65536)     53    49    48    52    93   161
+  //      4240  (16384)     40    36    28    27    39    60
+  //      8440  (16384)    117    82    58    49    49    70   129
+  //     16840  (16384)                 113    86    86    86   121
+  //     24532   (4096)                  93    64    52    49    56
+  //     42040  (65536)                      1409   877   887   873
+  //     84040   (2048)                              92    76    72
+  //    210040   (1024)                             157   119   111
+  // 16-bit elements go by the same bytes; theirs were not swept.
   if (tab.staged_bytes <= 640) return launch_rows<4, 64>(tab, stream);
   if (tab.staged_bytes <= 2048) return launch_rows<8, 128>(tab, stream);
   if (tab.staged_bytes <= 4096) return launch_rows<16, 128>(tab, stream);
   if (tab.staged_bytes <= 12288) return launch_rows<32, 128>(tab, stream);
   if (tab.staged_bytes <= 20480) return launch_rows<64, 64>(tab, stream);
   // Blocks of neighbouring elements in pairs, whose segments' ends meet in a line
-  // of L2: with up to twelve of them on an SM 42042 bytes 887 -> 869 us, 24534
-  // time-major 48.5 -> 44.6, batch-major 35.0 -> 33.4; with more (16842 bytes) the
+  // of L2: with up to twelve of them on an SM 42040 bytes 887 -> 869 us, 24532
+  // time-major 48.5 -> 44.6, batch-major 35.0 -> 33.4; with more (16840 bytes) the
   // scheduling of pairs costs more than that, 95 -> 110.
   if (tab.staged_bytes <= 65536) return launch_rows<128, 128>(tab, stream, 2);
   if (tab.staged_bytes <= 114688) return launch_rows<256, 256>(tab, stream);
   // Longer ones leave an SM one block, whose copies, sums and stores take turns:
   // blocks of a cluster share them. us in one block | 2 | 4 | 8:
-  //  84042 (2048)  72 | 79 | 90 | 134      210042 (1024)  111 | 105 | 103 | 104
+  //  84040 (2048)  72 | 79 | 90 | 134      210040 (1024)  111 | 105 | 103 | 104
   for (unsigned parts = 2; parts <= 8; parts *= 2)
     if (part_bytes(tab, parts) <= (parts < 8 ? 57344 : GRAD_MAX_STAGED))
       return launch_rows<128, 128, true>(tab, stream, parts);

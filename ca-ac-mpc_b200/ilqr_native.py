@@ -989,7 +989,7 @@ def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False):
     """Norm over all values of a sequence of gradients (float32, float16 or
     bfloat16, mixed as they come, any strides), a 0-d float32 tensor on their
     device; with per_tensor also each tensor's own norm, [n]. norm_type 2 or
-    inf. Nothing is read back to the host."""
+    inf. Nothing is read back to the host. The norms carry no autograd history."""
     got = (_binding_module or _binding()).grad_norm(grads, norm_type, True, per_tensor, False)
     return got if per_tensor else got[0]
 
@@ -1006,7 +1006,8 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 
     over all of them together (as grad_norm, or from `total`, a 0-d float64
     tensor on their device as grad_norm_total returns). Returns (the scaled
     gradients, norm): new tensors, or `out` where given; out=grads scales in
-    place. No output may share memory with another tensor of the call. A bound
+    place. No output may share memory with another tensor of the call, total
+    among them (a RuntimeError; outputs in each other's gaps share none). A bound
     of inf changes nothing; a NaN norm makes every value NaN, an infinite one 0
     or NaN. The outputs carry no autograd history."""
     return (_binding_module or _binding()).clip_grad_norm(grads, out, max_norm, norm_type, eps, total)
@@ -1015,11 +1016,12 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, eps: float = 
 def clip_grad_elements(grads, max_norm: float, batch_dims=0, eps: float = 1e-6, zero_nonfinite: bool = False, out=None):
     """Scale each batch element's gradient by itself: element b's gradient is
     its slices of up to eight tensors along their batch dimensions (one number
-    for all tensors, or one each; the time-major gradients of C and c have 1),
+    for all tensors, or one each, not negative; the time-major gradients of C
+    and c have 1),
     norms[b] the 2-norm over them, and they are scaled by
     min(1, max_norm / (norms[b] + eps)). The elements of a batch are separate
     solves, so one that diverges leaves the others' gradients as they are. Its
-    own become NaN (or 0, where its norm is infinite), or with zero_nonfinite
-    zero. Returns (the scaled gradients, norms [B] float32); out as in
-    clip_grad_norm."""
+    own become NaN (or, where its norm is infinite, 0 but for the infinities),
+    or with zero_nonfinite zero. Returns (the scaled gradients, norms [B]
+    float32); out as in clip_grad_norm."""
     return (_binding_module or _binding()).clip_grad_elements(grads, out, batch_dims, max_norm, eps, zero_nonfinite)
