@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <numeric>
 
 namespace ilqr {
 
@@ -46,11 +47,13 @@ class Meeting {
     m.above_ = -b.len;
     m.below_ = a.len;
     if (!m.add(a, -1) || !m.add(b, 1)) return true;
+    while (m.merge_one()) {}
     std::sort(m.s_, m.s_ + m.n_, [](const Step& x, const Step& y) { return x.stride > y.stride; });
-    m.min_[m.n_] = m.max_[m.n_] = 0;
+    m.min_[m.n_] = m.max_[m.n_] = m.measure_[m.n_] = 0;
     for (int k = m.n_ - 1; k >= 0; --k) {
       m.min_[k] = m.min_[k + 1] + m.s_[k].lo * m.s_[k].stride;
       m.max_[k] = m.max_[k + 1] + m.s_[k].hi * m.s_[k].stride;
+      m.measure_[k] = std::gcd(m.measure_[k + 1], m.s_[k].stride);
     }
     return m.reach(0, (int64_t)(b.base - a.base));
   }
@@ -61,10 +64,10 @@ class Meeting {
   };
   static constexpr int MAX_STEPS = 16;
   Step s_[MAX_STEPS];
-  int64_t min_[MAX_STEPS + 1], max_[MAX_STEPS + 1];
+  int64_t min_[MAX_STEPS + 1], max_[MAX_STEPS + 1], measure_[MAX_STEPS + 1];  // of the steps from k on
   int64_t above_ = 0, below_ = 0;
   int n_ = 0;
-  int tries_ = 4096;  // beyond them, and beyond MAX_STEPS, the answer is yes
+  int tries_ = 1 << 16;  // beyond them, and beyond MAX_STEPS, the answer is yes
 
   bool add(const Strided& r, int sign) {
     for (int k = 0; k < r.n; ++k) {
@@ -82,10 +85,28 @@ class Meeting {
     return true;
   }
 
+  // A stride of r smaller ones, whose own x fill the steps between its: together
+  // they take every multiple of the smaller stride in their range.
+  bool merge_one() {
+    for (int i = 0; i < n_; ++i)
+      for (int j = 0; j < n_; ++j) {
+        const int64_t r = s_[i].stride / s_[j].stride;
+        if (i == j || r * s_[j].stride != s_[i].stride || s_[j].hi - s_[j].lo < r - 1) continue;
+        s_[j].lo += r * s_[i].lo;
+        s_[j].hi += r * s_[i].hi;
+        s_[i] = s_[--n_];
+        return true;
+      }
+    return false;
+  }
+
   static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); }  // b > 0
 
   bool reach(int k, int64_t d) {
     if (k == n_) return d > above_ && d < below_;
+    // the first distance above the lower end that differs from d by whole measures
+    const int64_t off = (d - above_ - 1) % measure_[k];
+    if (above_ + 1 + off + (off < 0 ? measure_[k] : 0) >= below_) return false;
     const Step& s = s_[k];
     const int64_t first = std::max(s.lo, floor_div(above_ - d - max_[k + 1], s.stride) + 1);
     const int64_t last = std::min(s.hi, -floor_div(-(below_ - d - min_[k + 1]), s.stride) - 1);

@@ -158,3 +158,13 @@ def test_empty_tensors_of_every_shape():
                     _, n = nat.clip_grad_elements([empty], 1.0, batch_dims=dim, out=out and [empty])
                     assert n.tolist() == [0.0] * B
                     _check_elements([empty, x], [dim, 0], 1.5, out=out)
+
+
+def test_every_second_row_beside_all_rows():
+    base = _values((30_000, 64), F32, 2)
+    grads = [base[:, :32].t(), base[::2, 32:], base[1::2, 40:]]
+    left = base[1::2, 32:40].clone()
+    want = [t.clone() for t in nat.clip_grad_norm(grads, 3.0)[0]]
+    nat.clip_grad_norm(grads, 3.0, out=grads)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want)) and torch.equal(base[1::2, 32:40], left)
+    _refused(lambda: nat.clip_grad_norm(grads, 3.0, out=[grads[0], grads[1], base[::2, 40:]]), base)

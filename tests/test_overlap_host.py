@@ -153,3 +153,40 @@ def test_total_and_norm_beside_the_tensors_are_taken():
     for in_place in (True, False):
         assert _raw_elements(A + 4 * (210 * 79 + 14), in_place) == 4
         assert _raw_elements(A + 776, in_place) == 4                               # within a gap
+
+
+def test_long_sets_with_strides_of_their_own(meet):
+    """Every second row of a column beside all rows of another, and the like:
+    found for any number of rows."""
+    for N in (100, 20_000, 5_000_000, 2**40):
+        a = (1 << 20, 128, [(N, 256)])
+        for step in (2, 3, 17):
+            b = ((1 << 20) + 128, 128, [(N // step, 256 * step)])
+            assert not meet(a, b) and not meet(b, a)
+            assert meet(a, (b[0] + 1, 128, b[2])) and meet((b[0] - 1, 128, b[2]), a)
+        # blocks of rows, columns of each
+        c = (1 << 20, 64, [(N, 1024), (5, 192)])
+        d = ((1 << 20) + 64, 128, [(N // 3, 3072), (4, 192)])
+        assert not meet(c, d) and not meet(d, c) and meet(c, (d[0], 129, d[2]))
+    # strides without a common measure: the first two runs that meet are far on
+    for s, t, n in ((1009, 1013, 1013), (10_007, 10_009, 10_009)):
+        a, b = (0, 1, [(n, s)]), (5, 1, [(n, t)])
+        # i s = 5 + j t with 0 <= i, j < n
+        j = next((j for j in range(n) if (5 + j * t) % s == 0 and (5 + j * t) // s < n), None)
+        assert j is not None and meet(a, b)
+        assert not meet((0, 1, [((5 + j * t) // s, s)]), (5, 1, [(j + 1, t)]))
+
+
+def test_larger_sets_against_their_addresses(meet):
+    rng = random.Random(11)
+    seen = [0, 0]
+    for _ in range(1500):
+        sets = []
+        unit = rng.choice([1, 1, 2, 7, 16])
+        for _ in range(2):
+            dims = [(rng.randint(1, 40), rng.randint(1, 60) * unit) for _ in range(rng.randint(1, 2))]
+            sets.append((5000 + rng.randint(0, 700), rng.randint(1, 3), dims))
+        want = bool(_bytes(sets[0]) & _bytes(sets[1]))
+        assert meet(*sets) == want and meet(*reversed(sets)) == want, sets
+        seen[want] += 1
+    assert min(seen) > 100
